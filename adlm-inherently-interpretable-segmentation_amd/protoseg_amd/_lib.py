@@ -9,6 +9,7 @@ HIP calls to that same runtime, so stream handles from ``torch.cuda`` are valid 
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import pathlib
@@ -32,7 +33,8 @@ OPERANDS_READY = 0x200  # OR-ed into protoseg_l2_fwd_ex's act_kind: operands hol
 PREC_BF16X3, PREC_BF16X6, PREC_F32 = 0, 1, 2
 PRECISIONS = {"bf16x3": PREC_BF16X3, "bf16x6": PREC_BF16X6, "f32": PREC_F32}
 
-_vp, _i, _f, _sz, _i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_int64
+_vp, _i, _f, _d, _sz, _i64 = (ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_double, ctypes.c_size_t,
+                              ctypes.c_int64)
 
 # name -> (restype, argtypes); exactly the symbols declared in include/protoseg_hip.h
 SIGNATURES = {
@@ -48,6 +50,10 @@ SIGNATURES = {
     "protoseg_l2_bwd_saved": (_i, [_vp, _i, _i, _i, _i, _i, _vp, _i, _vp, _i, _f, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp,
                                    _vp, _sz, _vp]),
     "protoseg_adam_step": (_i, [_i, _vp, _vp, _vp, _vp, _vp, _vp, _f, _f, _f, _f, _f, _vp]),
+    "protoseg_group_norm_workspace_size": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "protoseg_group_norm_fwd": (_i, [_vp, _i, _i, _i, _i, _i64, _i64, _i, _vp, _vp, _d, _i, _vp, _vp, _vp, _sz, _vp]),
+    "protoseg_group_norm_bwd": (_i, [_vp, _vp, _i, _i, _i, _i, _i64, _i64, _i64, _i64, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp,
+                                     _vp, _sz, _vp]),
     "protoseg_l2_adam_prep_supported": (_i, [_i, _i, _i, _i]),
     "protoseg_l2_adam_prep": (_i, [_i, _i, _i, _f, _i, _i, _vp, _vp, _vp, _vp, _vp, _f, _f, _vp, _vp, _vp, _vp, _vp, _f,
                                    _f, _f, _f, _f, _vp, _sz, _vp]),
@@ -125,10 +131,13 @@ def load() -> ctypes.CDLL:
 
 def call(name: str, *args) -> None:
     """Calls an int-status entry point and raises ProtosegError on failure."""
-    lib = load()
-    status = getattr(lib, name)(*args)
+    check(name, getattr(load(), name)(*args))
+
+
+def check(name: str, status: int) -> None:
+    """Raises ProtosegError for the status that entry point ``name`` returned, unless it is OK."""
     if status != OK:
-        msg = lib.protoseg_last_error()
+        msg = load().protoseg_last_error()
         raise ProtosegError(f"{name} failed with status {status}: {msg.decode() if msg else ''}")
 
 
@@ -143,8 +152,21 @@ def ptr(t: torch.Tensor | None) -> ctypes.c_void_p:
     return ctypes.c_void_p(t.data_ptr())
 
 
+def addr(t: torch.Tensor | None) -> int | None:
+    """Device address of a tensor as a plain integer (None: NULL)."""
+    return None if t is None else t.data_ptr()
+
+
 def stream_of(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """``torch.cuda.device(device)``, without its cost where the device is the current one already."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def require_device(*tensors: torch.Tensor) -> torch.device:

@@ -575,6 +575,31 @@ int protoseg_l2_adam_prep(int C, int P, int K, float eps, int act_kind, int prec
                           float beta1, float beta2, float adam_eps,
                           void* operands, size_t operands_bytes, protoseg_stream_t stream);
 
+/*
+ * Group norm with an activation on channels-last maps: the normalisation that trains at the
+ * reference's micro-batch of 2 (it freezes BatchNorm there, segmentation/module.py:127).
+ *   x    element (b, pixel, c) at x[b * stride_b + pixel * stride_pixel + c] (strides in elements,
+ *        stride_pixel >= C), x_dtype F32, BF16 or F16
+ *   weight, bias  [C] f32, or NULL (1 and 0)
+ *   y    [B, HW, C] dense, x's dtype: act((x - mean) rstd weight + bias), statistics per (sample,
+ *        group of C / groups channels) over all pixels, rstd = 1 / sqrt(var + eps)
+ *   stats [B, groups, 2] f64: mean, rstd (the backward reads them)
+ *   act_kind  0 identity, 1 relu, 2 sigmoid, 3 silu
+ * The backward writes g_x [B, HW, C] dense (x's dtype), g_weight and g_bias [C] f32 (overwritten),
+ * each of them optional (NULL). g_y: x's dtype, strides of its own. Results do not depend on the
+ * schedule (no atomics). workspace: protoseg_group_norm_workspace_size(...) bytes, 256-B aligned,
+ * of one call at a time. B == 0 or HW == 0: nothing is read, g_weight and g_bias are zeroed.
+ */
+size_t protoseg_group_norm_workspace_size(int x_dtype, int B, int HW, int C, int groups, int backward);
+int protoseg_group_norm_fwd(const void* x, int x_dtype, int B, int HW, int C, int64_t stride_b, int64_t stride_pixel,
+                            int groups, const float* weight, const float* bias, double eps, int act_kind, void* y,
+                            double* stats, void* workspace, size_t workspace_bytes, protoseg_stream_t stream);
+int protoseg_group_norm_bwd(const void* x, const void* g_y, int x_dtype, int B, int HW, int C, int64_t stride_b,
+                            int64_t stride_pixel, int64_t g_stride_b, int64_t g_stride_pixel, int groups,
+                            const float* weight, const float* bias, int act_kind, const double* stats, void* g_x,
+                            float* g_weight, float* g_bias, void* workspace, size_t workspace_bytes,
+                            protoseg_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
