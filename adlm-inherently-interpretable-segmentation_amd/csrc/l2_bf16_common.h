@@ -115,6 +115,19 @@ __device__ __forceinline__ void dma(rsrc_t r, void* lds, unsigned voff, unsigned
                  : "memory");
 }
 
+// 16-B LDS-DMA of one wave-instruction (1 KiB, lane-linear at lds + 16 lane); out-of-range
+// lanes land as zeros. Inline asm so the compiler does not drain it before unrelated LDS reads
+// (the dma<> note above); the kernel waits for it itself.
+__device__ __forceinline__ void dma16(rsrc_t r, unsigned lds, unsigned voff, unsigned soff) {
+  unsigned so = __builtin_amdgcn_readfirstlane(soff);
+  asm volatile("" : "+s"(so));
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep)
+               : "v"(voff), "s"(__builtin_amdgcn_readfirstlane(lds)), "s"(r), "s"(so)
+               : "memory");
+}
+
 // ||x||^2 of one pixel in the bf16 family's fixed order: s_{q,h} = fma chain over the 8
 // channels chan_of(q, h, 0..7) starting from 0, u_q = s_{q,0} + s_{q,1}, and
 // x2 = (u_0 + u_1) + (u_2 + u_3). Every kernel of the family that needs ||x||^2 (forward,

@@ -873,18 +873,7 @@ __global__ __launch_bounds__(256) void wide_f16_prep_kernel(const float* __restr
   }
 }
 
-// 16-B LDS-DMA of one wave-instruction (1 KiB, lane-linear at lds + 16 lane); out-of-range
-// lanes land as zeros. Inline asm so the compiler does not drain it before unrelated LDS reads
-// (the dma<> note in l2_bf16_common.h); the kernel waits for it itself.
-__device__ __forceinline__ void dma16(rsrc_t r, unsigned lds, unsigned voff, unsigned soff) {
-  unsigned so = __builtin_amdgcn_readfirstlane(soff);
-  asm volatile("" : "+s"(so));
-  unsigned keep;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
-               : "=&s"(keep)
-               : "v"(voff), "s"(__builtin_amdgcn_readfirstlane(lds)), "s"(r), "s"(so)
-               : "memory");
-}
+using bf16l::dma16;
 
 // x stage image: 256-B rows (one channel, 128 pixels), 16-B chunk ch of row r at
 // 256 r + 16 (ch ^ swz) (cdna_hip_programming.md T10 image (b): the transposed reads of the

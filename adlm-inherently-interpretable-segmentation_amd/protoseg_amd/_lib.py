@@ -54,6 +54,10 @@ SIGNATURES = {
     "protoseg_group_norm_fwd": (_i, [_vp, _i, _i, _i, _i, _i64, _i64, _i, _vp, _vp, _d, _i, _vp, _vp, _vp, _sz, _vp]),
     "protoseg_group_norm_bwd": (_i, [_vp, _vp, _i, _i, _i, _i, _i64, _i64, _i64, _i64, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp,
                                      _vp, _sz, _vp]),
+    "protoseg_orthogonalize_workspace_size": (_sz, [_i, _i, _i]),
+    "protoseg_orthogonalize": (_i, [_vp, _i, _i, _i, _i, _i64, _i, _f, _f, _f, _f, _vp, _vp, _sz, _vp]),
+    "protoseg_muon_workspace_size": (_sz, [_i, _vp, _vp]),
+    "protoseg_muon_step": (_i, [_i, _vp, _vp, _vp, _vp, _vp, _f, _i, _f, _f, _i, _i, _f, _f, _f, _f, _vp, _sz, _vp]),
     "protoseg_l2_adam_prep_supported": (_i, [_i, _i, _i, _i]),
     "protoseg_l2_adam_prep": (_i, [_i, _i, _i, _f, _i, _i, _vp, _vp, _vp, _vp, _vp, _f, _f, _vp, _vp, _vp, _vp, _vp, _f,
                                    _f, _f, _f, _f, _vp, _sz, _vp]),

@@ -166,3 +166,140 @@ class Adam(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)
         self._steps = {}  # re-seeded from the loaded state[p]['step'] at the next step()
+
+
+# a, b, c of the quintic s -> a s + b s^3 + c s^5 that Muon iterates: the steepest at 0 that keeps [0, 1]
+# near 1 after five steps (singular values end between about 0.7 and 1.2, not at 1)
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+_MUON_SCALES = {"original": 0, "rms": 1}
+
+
+def _matrix_dtype(t: torch.Tensor) -> int:
+    code = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}.get(t.dtype)
+    if code is None:
+        raise _lib.ProtosegError(f"orthogonalize dtype {t.dtype} unsupported (float32, bfloat16 or float16)")
+    return code
+
+
+@torch.no_grad()
+def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 1e-7) -> torch.Tensor:
+    """The matrices g [..., rows, cols] with their singular values pushed towards 1 by ``steps``
+    Newton-Schulz steps X <- a X + b (X X^T) X + c (X X^T)^2 X from X = g / (|g|_F + eps)
+    (``protoseg_orthogonalize``: f32-class arithmetic, the result rounded once to g's dtype). No gradient.
+
+    g: float32, bfloat16 or float16; matrices with dense rows at a constant distance are read in
+    place, other layouts are copied once. The result is dense. Coefficients that let a singular value
+    grow to 4 are refused.
+    """
+    code = _matrix_dtype(g)
+    if g.dim() < 2:
+        raise _lib.ProtosegError(f"orthogonalize takes [..., rows, cols]; got {tuple(g.shape)}")
+    dev = _lib.require_device(g)
+    rows, cols = g.shape[-2:]
+    a, b, c = (float(v) for v in coefficients)
+    out = torch.empty(g.shape, dtype=g.dtype, device=dev)
+    m = g if g.dim() == 3 else g.reshape(-1, rows, cols) if g.numel() else g.new_empty((0, rows, cols))
+    count = m.shape[0]
+    dense = (cols == 1 or m.stride(2) == 1) and (rows == 1 or m.stride(1) == cols)
+    if not dense or (count > 1 and m.stride(0) < rows * cols):
+        m = m.contiguous()
+    stride = m.stride(0) if count > 1 else rows * cols
+    lib = _lib.load()
+    with _lib.on_device(dev):
+        nbytes = lib.protoseg_orthogonalize_workspace_size(count, rows, cols)
+        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        _lib.check("protoseg_orthogonalize", lib.protoseg_orthogonalize(
+            m.data_ptr(), code, count, rows, cols, stride, int(steps), a, b, c, float(eps), out.data_ptr(), ws.data_ptr(),
+            nbytes, _lib.stream_of(dev)))
+    return out
+
+
+class Muon(torch.optim.Optimizer):
+    """Momentum with orthogonalised updates (``protoseg_muon_step``), for parameters that are matrices:
+
+        B <- momentum B + g;   U = g + momentum B (nesterov) or B
+        p <- (1 - lr weight_decay) p - lr s orthogonalize(U)
+
+    A parameter of more than two dimensions is the matrix [size(0), rest]: a convolution's weight, the
+    prototype vectors [P, C, 1, 1]. ``scale``: "original", s = sqrt(max(1, rows / cols)), or "rms",
+    s = 0.2 sqrt(max(rows, cols)) (the update's root mean square then is about Adam's). Biases and other vectors belong to
+    ``Adam``; ``train.PatchClassificationStep`` steps a list of optimizers. All tensors of a group share
+    the launches, and a HIP graph holding ``step()`` replays as successive steps. float32 on the GPU only.
+    """
+
+    def __init__(self, params: Iterable, lr: float = 2e-2, momentum: float = 0.95, nesterov: bool = True,
+                 weight_decay: float = 0.0, ns_steps: int = 5, ns_coefficients=NS_COEFFICIENTS, eps: float = 1e-7,
+                 scale: str = "original"):
+        if lr < 0 or eps < 0 or weight_decay < 0 or not 0 <= momentum < 1 or scale not in _MUON_SCALES:
+            raise ValueError("invalid Muon hyper-parameters")
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
+                                      ns_steps=ns_steps, ns_coefficients=tuple(ns_coefficients), eps=eps, scale=scale))
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.dim() < 2:
+                    raise ValueError(f"Muon takes matrices; got a parameter of shape {tuple(p.shape)}")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            ps, gs, bufs, rows, cols = [], [], [], [], []
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                r = p.shape[0]
+                n = p.numel()
+                if p.dtype != torch.float32 or p.grad.dtype != torch.float32 or p.grad.is_sparse or p.dim() < 2:
+                    raise _lib.ProtosegError("protoseg Muon: float32 matrices and dense gradients only")
+                st = self.state[p]
+                if "momentum_buffer" not in st:
+                    st["momentum_buffer"] = torch.zeros_like(p)
+                buf, g = st["momentum_buffer"], p.grad
+                if not _dense_rows(p):
+                    raise _lib.ProtosegError(f"protoseg Muon: parameter of strides {p.stride()} is not dense row by row")
+                if buf.stride() != p.stride() or buf.dtype != torch.float32 or buf.shape != p.shape:
+                    # (a loaded state of another layout) the columns of p, g and B have to be in one order
+                    buf = st["momentum_buffer"] = torch.empty_like(p).copy_(buf)
+                if g.stride() != p.stride():
+                    g = torch.empty_like(p).copy_(g)
+                if n:
+                    ps.append(p)
+                    gs.append(g)
+                    bufs.append(buf)
+                    rows.append(r)
+                    cols.append(n // r)
+            if not ps:
+                continue
+            dev = _lib.require_device(*ps, *gs, *bufs)
+            k = len(ps)
+            arrays = [(ctypes.c_void_p * k)(*[t.data_ptr() for t in ts]) for ts in (ps, gs, bufs)]
+            arrays += [(ctypes.c_int32 * k)(*v) for v in (rows, cols)]
+            addr = [ctypes.cast(a, ctypes.c_void_p) for a in arrays]
+            a, b, c = (float(v) for v in group["ns_coefficients"])
+            lib = _lib.load()
+            with _lib.on_device(dev):
+                nbytes = lib.protoseg_muon_workspace_size(k, addr[3], addr[4])
+                ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+                _lib.check("protoseg_muon_step", lib.protoseg_muon_step(
+                    k, *addr, float(group["momentum"]), int(bool(group["nesterov"])), float(group["lr"]),
+                    float(group["weight_decay"]), _MUON_SCALES[group["scale"]], int(group["ns_steps"]), a, b, c,
+                    float(group["eps"]), ws.data_ptr(), nbytes, _lib.stream_of(dev)))
+        return loss
+
+
+def _dense_rows(p: torch.Tensor) -> bool:
+    """Whether p's memory is p.shape[0] rows back to back, each dense in some order of its dimensions
+    (contiguous, and a channels-last convolution weight)."""
+    if p.is_contiguous():
+        return True
+    r = p.shape[0]
+    rest = sorted((s, n) for s, n in zip(p.stride()[1:], p.shape[1:]) if n > 1)
+    at = 1
+    for s, n in rest:
+        if s != at:
+            return False
+        at *= n
+    return r == 1 or p.stride(0) == at

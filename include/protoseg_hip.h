@@ -600,6 +600,38 @@ int protoseg_group_norm_bwd(const void* x, const void* g_y, int x_dtype, int B, 
                             float* g_weight, float* g_bias, void* workspace, size_t workspace_bytes,
                             protoseg_stream_t stream);
 
+/*
+ * Orthogonalising matrices by Newton-Schulz products: for each of `count` matrices g [rows, cols]
+ * (dense rows; matrix i at g + i * stride elements), X0 = g / (|g|_F + eps), then `steps` (1..32) times
+ *   X <- a X + b (X X^T) X + c (X X^T)^2 X
+ * (for rows > cols on the transpose), i.e. every singular value s goes to a s + b s^3 + c s^5.
+ *   dtype  F32, BF16 or F16; out [count, rows, cols] dense, of the same dtype (may not overlap g)
+ * Arithmetic: f32-class (f16 pairs, f32 accumulation) for every dtype; a 16-bit result is rounded once. A zero
+ * matrix gives zeros; a value that is not finite makes its own matrix NaN. Coefficients under which a
+ * singular value in [0, 1] could grow to 4 are refused (PROTOSEG_ERR_UNSUPPORTED). No atomics: the same bits
+ * on every run. workspace: protoseg_orthogonalize_workspace_size(...) bytes, 256-B aligned, of one call
+ * at a time.
+ */
+size_t protoseg_orthogonalize_workspace_size(int count, int rows, int cols);
+int protoseg_orthogonalize(const void* g, int dtype, int count, int rows, int cols, int64_t stride, int steps, float a,
+                           float b, float c, float eps, void* out, void* workspace, size_t workspace_bytes,
+                           protoseg_stream_t stream);
+
+/*
+ * Muon optimizer step of n_tensors f32 matrices (host arrays of device pointers, rows[k] x cols[k] dense):
+ *   B <- momentum B + g;   U = g + momentum B (nesterov) or B
+ *   p <- (1 - lr weight_decay) p - lr s orthogonalize(U)
+ * with s = sqrt(max(1, rows / cols)) (scale_kind 0) or 0.2 sqrt(max(rows, cols)) (scale_kind 1), and
+ * steps, a, b, c, eps as protoseg_orthogonalize. momentum_bufs[k] is B, updated in place. All tensors share
+ * the launches (24 shapes a run); kernel launches only, so the call can be captured. A tensor may
+ * appear once.
+ */
+size_t protoseg_muon_workspace_size(int n_tensors, const int32_t* rows, const int32_t* cols);
+int protoseg_muon_step(int n_tensors, float* const* params, const float* const* grads, float* const* momentum_bufs,
+                       const int32_t* rows, const int32_t* cols, float momentum, int nesterov, float lr,
+                       float weight_decay, int scale_kind, int steps, float a, float b, float c, float eps,
+                       void* workspace, size_t workspace_bytes, protoseg_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
