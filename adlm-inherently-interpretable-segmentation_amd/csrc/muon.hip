@@ -22,6 +22,7 @@
 // covers all groups. Matrices are padded to 64 rows and columns with zeros, so the products have no edges.
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 #include <utility>
 #include <vector>
@@ -44,6 +45,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 constexpr int kPad = 64;
 constexpr int kMaxGroups = 24, kMaxItems = 32, kMaxSteps = 32;
 constexpr float kScale = 1024.f;  // of X, A and T: entries below 16 (checked) stay below 2^14
+constexpr long long kBigTiles = 192;
 constexpr int kNormThreads = 256, kMaxChunks = 256;
 constexpr long long kNormLeast = 16384;  // elements per workgroup of the sums of squares
 
@@ -336,11 +338,13 @@ __global__ __launch_bounds__(256, 1) void ns_product_kernel(NsGroups gs, NsJobs 
 
   const int wi = (wave & 1) * (T / 2), wc = (wave >> 1) * (T / 2);
   const int gq = lane >> 4, q4 = (lane >> 2) & 3, p4 = lane & 3;
-  f32x16 acc[MI][MI];
+  // hi hi, and the cross terms apart: they are 2^-11 of it, and a sum of their own takes two of every three
+  // roundings out of the large one
+  f32x16 acc[MI][MI], cross[MI][MI];
 #pragma unroll
   for (int a = 0; a < MI; ++a)
 #pragma unroll
-    for (int b = 0; b < MI; ++b) acc[a][b] = zero16();
+    for (int b = 0; b < MI; ++b) acc[a][b] = cross[a][b] = zero16();
 
   if (nst > 0) issue(0);
   if (nst > 1) issue(1);
@@ -355,18 +359,17 @@ __global__ __launch_bounds__(256, 1) void ns_product_kernel(NsGroups gs, NsJobs 
     }
     if (st + 2 < nst) issue(st + 2);  // into the stage that every wave has read before this barrier
     const unsigned sb = S0 + static_cast<unsigned>((st % kStages) * stage_bytes(T));
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      f16x8 lf[MI][2], rf[MI][2];
+    f16x8 lf[2][MI][2], rf[2][MI][2];
+    auto read_step = [&](int ks) __attribute__((always_inline)) {
 #pragma unroll
       for (int a = 0; a < MI; ++a) {
         const int r = wi + 32 * a + j, c = wc + 32 * a + j;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          lf[a][t] = *reinterpret_cast<const __attribute__((address_space(3))) f16x8*>(static_cast<uintptr_t>(
+          lf[ks][a][t] = *reinterpret_cast<const __attribute__((address_space(3))) f16x8*>(static_cast<uintptr_t>(
               sb + static_cast<unsigned>(t * kPlane + r * 64 + 16 * ((2 * ks + h) ^ nt_swz(r)))));
           if constexpr (!KX) {
-            rf[a][t] = *reinterpret_cast<const __attribute__((address_space(3))) f16x8*>(static_cast<uintptr_t>(
+            rf[ks][a][t] = *reinterpret_cast<const __attribute__((address_space(3))) f16x8*>(static_cast<uintptr_t>(
                 sb + static_cast<unsigned>((2 + t) * kPlane + c * 64 + 16 * ((2 * ks + h) ^ nt_swz(c)))));
           } else {
             s16x4 v[2];
@@ -377,26 +380,44 @@ __global__ __launch_bounds__(256, 1) void ns_product_kernel(NsGroups gs, NsJobs 
                   static_cast<uintptr_t>(sb + static_cast<unsigned>((2 + t) * kPlane + kr * (2 * T) +
                                                                     16 * (ch ^ kx_swz<T>(kr)) + 8 * (p4 & 1)))));
             }
-            rf[a][t] = __builtin_bit_cast(f16x8, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+            rf[ks][a][t] = __builtin_bit_cast(f16x8, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
           }
         }
       }
+    };
+    // kTall: the transposed block, so that lanes run along the result's rows
+    auto mma = [&](f32x16 (&d)[MI][MI], int ks, int tl, int tr) __attribute__((always_inline)) {
 #pragma unroll
       for (int a = 0; a < MI; ++a)
 #pragma unroll
         for (int b = 0; b < MI; ++b) {
-          auto mma = [&](int tl, int tr) {  // kTall: the transposed block, so that lanes run along the result's rows
-            if constexpr (MODE == kTall)
-              acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(rf[b][tr], lf[a][tl], acc[a][b], 0, 0, 0);
-            else
-              acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lf[a][tl], rf[b][tr], acc[a][b], 0, 0, 0);
-          };
-          mma(1, 0);
-          mma(0, 1);
-          mma(0, 0);
+          if constexpr (MODE == kTall)
+            d[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(rf[ks][b][tr], lf[ks][a][tl], d[a][b], 0, 0, 0);
+          else
+            d[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lf[ks][a][tl], rf[ks][b][tr], d[a][b], 0, 0, 0);
         }
+    };
+    // the first 16 k's fragments, then one read of the second's behind each of the first's products
+    read_step(0);
+    __builtin_amdgcn_sched_barrier(0);
+    read_step(1);
+    mma(cross, 0, 1, 0);
+    mma(cross, 0, 0, 1);
+    mma(acc, 0, 0, 0);
+#pragma unroll
+    for (int k = 0; k < (KX ? 6 : 4) * MI; ++k) {
+      if (k < 3 * MI * MI) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // one MFMA
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                       // one LDS read
     }
+    __builtin_amdgcn_sched_barrier(0);
+    mma(cross, 1, 1, 0);
+    mma(cross, 1, 0, 1);
+    mma(acc, 1, 0, 0);
   }
+#pragma unroll
+  for (int a = 0; a < MI; ++a)
+#pragma unroll
+    for (int b = 0; b < MI; ++b) acc[a][b] += cross[a][b];
 
 #pragma unroll
   for (int a = 0; a < MI; ++a)
@@ -486,31 +507,39 @@ __global__ __launch_bounds__(256, 1) void ns_product_kernel(NsGroups gs, NsJobs 
     }
 }
 
-// The partials of a split Gram product joined in a fixed order, one 32 x 32 block (on or above the
-// diagonal) a wave, stored with its mirror image.
+// The partials of a split Gram product joined in a fixed order: a workgroup takes one 32 x 32 block on or
+// above the diagonal, each wave every fourth split, and stores it with its mirror image.
 __global__ __launch_bounds__(256) void ns_join_kernel(NsGroups gs, float inv, int grown) {
+  __shared__ float red[3][16][64];
   const NsGroup& g = gs.g[group_of(gs, blockIdx.x)];
-  const int nb = g.mp / 32, tri = nb * (nb + 1) / 2, per = (tri + 3) / 4;
+  const int nb = g.mp / 32, per = nb * (nb + 1) / 2;
   const int local = static_cast<int>(blockIdx.x) - g.first, mat = local / per;
-  int blk = (local - mat * per) * 4 + bf16l::wave_id(), bi = 0;
-  if (blk >= tri) return;
+  int blk = local - mat * per, bi = 0;
   while (blk >= nb - bi) blk -= nb - bi, ++bi;
-  const int bc = bi + blk, lane = threadIdx.x & 63, j = lane & 31, h = lane >> 5;
+  const int bc = bi + blk, lane = threadIdx.x & 63, wave = bf16l::wave_id(), j = lane & 31, h = lane >> 5;
   const long long psz = static_cast<long long>(g.mp) * g.mp;
-  inv = ldexpf(inv, -2 * x_shift(target_of(gs, g, mat), grown));
-  const float* src = reinterpret_cast<const float*>(gs.ws + g.part) + static_cast<long long>(mat) * g.split * psz;
+  const float* src = reinterpret_cast<const float*>(gs.ws + g.part) + static_cast<long long>(mat) * g.split * psz +
+                     static_cast<long long>(32 * bi + 4 * h) * g.mp + 32 * bc + j;
   float v[16];
 #pragma unroll
   for (int r = 0; r < 16; ++r) v[r] = 0.f;
-  for (int z = 0; z < g.split; ++z) {
+#pragma unroll 4
+  for (int z = wave; z < g.split; z += 4) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) v[r] += src[z * psz + static_cast<long long>(32 * bi + acc_row(r, h)) * g.mp + 32 * bc + j];
+    for (int r = 0; r < 16; ++r) v[r] += src[z * psz + static_cast<long long>(row_of(r)) * g.mp];
   }
+  if (wave) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) red[wave - 1][r][lane] = v[r];
+  }
+  __syncthreads();
+  if (wave) return;
+  inv = ldexpf(inv, -2 * x_shift(target_of(gs, g, mat), grown));
   _Float16* hi = plane_of(gs, g, kA, mat);
   Pair p[16];
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    p[r] = split_pair(v[r] * inv);
+    p[r] = split_pair((((v[r] + red[0][r][lane]) + red[1][r][lane]) + red[2][r][lane]) * inv);
     const long long at = static_cast<long long>(32 * bi + acc_row(r, h)) * g.mp + 32 * bc + j;
     hi[at] = p[r].hi;
     hi[psz + at] = p[r].lo;
@@ -615,6 +644,14 @@ size_t ns_layout(NsGroups& gs, const std::vector<NsMatrix>& mats, std::vector<in
     }
     gs.g[k].count += mats[i].count;
   }
+  // the matrices with the most work a tile first, so that a launch does not end on them
+  std::vector<int> order(gs.n), place(gs.n);
+  for (int k = 0; k < gs.n; ++k) order[k] = k;
+  std::stable_sort(order.begin(), order.end(), [&](int p, int q) { return gs.g[p].mp > gs.g[q].mp; });
+  const NsGroups was = gs;
+  for (int k = 0; k < gs.n; ++k) gs.g[k] = was.g[order[k]], place[order[k]] = k;
+  if (which)
+    for (int& w : *which) w = place[w];
   long long tiles = 0;  // 64 x 64 Gram tiles in all
   for (int k = 0; k < gs.n; ++k) tiles += static_cast<long long>(gs.g[k].count) * (gs.g[k].mp / 64) * (gs.g[k].mp / 64 + 1) / 2;
   long long at = 0, total = 0;
@@ -628,7 +665,7 @@ size_t ns_layout(NsGroups& gs, const std::vector<NsMatrix>& mats, std::vector<in
     // The Gram contraction is split where it is long (a split is at least 8 stages) and the launch has
     // fewer tiles than the chip has places for, or its chain of stages would outlast everything else's.
     const long long stages = g.np / 32;
-    long long split = 768 / (tiles < 1 ? 1 : tiles) + 1;
+    long long split = 384 / (tiles < 1 ? 1 : tiles);
     const long long chain = (stages + 63) / 64, most = stages / 8;
     if (split < chain) split = chain;
     if (split > most) split = most;
@@ -688,9 +725,8 @@ int ns_launch(NsGroups gs, const NsJobs& js, hipStream_t st) {
 }
 
 // All products of a prepared X0, ending in the targets.
-template <int OUT>
+template <int T, int OUT>
 int ns_products(NsGroups gs, const NsPlan& pl, hipStream_t st) {
-  constexpr int T = 64;
   int x = kX0, step = 0;
   auto sym = [&](std::initializer_list<NsJob> jobs, int partial = 0) {
     NsJobs js{};
@@ -706,7 +742,7 @@ int ns_products(NsGroups gs, const NsPlan& pl, hipStream_t st) {
       NsGroups js = gs;
       const long long blocks = ns_grid(js, [](const NsGroup& g) -> long long {
         const long long nb = g.mp / 32;
-        return g.split > 1 ? ceil_div(nb * (nb + 1) / 2, 4) : 0;
+        return g.split > 1 ? nb * (nb + 1) / 2 : 0;
       });
       hipLaunchKernelGGL(ns_join_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, js, 1.f / kScale, pl.grown[p]);
       if (int e = check_launch("ns_join_kernel")) return e;
@@ -747,6 +783,16 @@ int ns_products(NsGroups gs, const NsPlan& pl, hipStream_t st) {
     }
   }
   return PROTOSEG_OK;
+}
+
+template <int OUT>
+int ns_products(const NsGroups& gs, const NsPlan& pl, hipStream_t st) {
+  long long tiles = 0;
+  for (int k = 0; k < gs.n; ++k) {
+    const long long nt = ceil_div(gs.g[k].mp, 128);
+    tiles += nt * (nt + 1) / 2 * gs.g[k].count;
+  }
+  return tiles >= kBigTiles ? ns_products<128, OUT>(gs, pl, st) : ns_products<64, OUT>(gs, pl, st);
 }
 
 // Sums of squares and X0 of all items, kMaxItems a launch.
