@@ -58,17 +58,19 @@ struct NsTarget {
   int small;         // X0's norm is at most 2^-small (above 0 where eps outweighs |G|)
 };
 
-// One shape. Buffers (byte offsets from the workspace; every matrix a hi plane and a lo plane, row-major):
-// X0, X1 [count][2][mp][np] f16 at x; A, P, T, Q0, Q1 [count][2][mp][mp] f16 at sq; Gram partials
-// [count][split][mp][mp] f32 at part.
+// One shape. Buffers (byte offsets from the workspace): X0, X1 [count][mp][np] pairs at x; A, P, T, Q0, Q1
+// [count][mp][mp] pairs at sq; Gram partials [count][split][mp][mp] f32 at part. Pairs are row-major, 32 hi
+// values and their 32 lo values in turn: a 32-k stage of a row is one 128-B line (with hi and lo in planes
+// of their own it was two half lines, and L2 served twice the requests).
 struct NsGroup {
   int m, n, mp, np, count, tall;
-  int split, first;  // workgroups along the Gram contraction; first workgroup of the group in this launch
+  int split;         // workgroups along the Gram contraction
   int chunks, target;  // chunks of the sums of squares; index of the first matrix's NsTarget and sums
   long long x, sq, part;
 };
 struct NsGroups {
   NsGroup g[kMaxGroups];
+  int first[kMaxGroups];  // first workgroup of each group in this launch (no workgroup's from n on)
   int n;
   unsigned char* ws;
   long long targets, sums;  // byte offsets: NsTarget[matrices], double[matrices][kMaxChunks]
@@ -80,21 +82,28 @@ struct NsItem {
   const void* src;
   float *p, *buf;     // kOutStep: parameters and momentum; else p is the output
   long long sb, ob;   // elements from matrix to matrix
-  int count, group, index;  // the item's first matrix is the group's `index`
-  int first;
+  int count, rows, cols;
+  int group, index;  // the item's first matrix is the group's `index` (ns_small_kernel has no groups)
   float rate, keep;
 };
 struct NsItems {
   NsItem it[kMaxItems];
+  int first[kMaxItems];
   int n;
 };
 
 __device__ __forceinline__ long long x_bytes(const NsGroup& g) { return 4LL * g.mp * g.np; }
 __device__ __forceinline__ long long sq_bytes(const NsGroup& g) { return 4LL * g.mp * g.mp; }
-__device__ __forceinline__ _Float16* plane_of(const NsGroups& gs, const NsGroup& g, int buf, int mat) {
+__device__ __forceinline__ _Float16* pairs_of(const NsGroups& gs, const NsGroup& g, int buf, int mat) {
   const long long o = buf <= kX1 ? g.x + (static_cast<long long>(buf) * g.count + mat) * x_bytes(g)
                                  : g.sq + (static_cast<long long>(buf - kA) * g.count + mat) * sq_bytes(g);
   return reinterpret_cast<_Float16*>(gs.ws + o);
+}
+
+// hi of element (row, col) of a matrix of `ld` columns; lo is kLo further.
+constexpr int kLo = 32;
+__device__ __forceinline__ long long at_pair(int row, int col, int ld) {
+  return static_cast<long long>(row) * (2 * ld) + (col >> 5) * 64 + (col & 31);
 }
 
 struct Pair {
@@ -107,20 +116,40 @@ __device__ __forceinline__ Pair split_pair(float v) {
   return p;
 }
 
+// A 32 x 32 block of a product (lane: one column, acc_row's rows) as pairs at `dst`, the block's first hi.
+// (8-B stores after a 4 x 4 exchange within quads measured 10 to 15 % slower over whole launches: the
+// exchange is vector work of every wave.)
+__device__ __forceinline__ void store_block(_Float16* dst, const Pair (&p)[16], int ld, int lane) {
+  const int j = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const long long at = static_cast<long long>(acc_row(r, h)) * (2 * ld) + j;
+    dst[at] = p[r].hi;
+    dst[at + kLo] = p[r].lo;
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ float src_at(const void* p, long long i) {
   return static_cast<float>(static_cast<const T*>(p)[i]);
 }
 
-__device__ __forceinline__ int item_of(const NsItems& its, int blk) {
+// The group (item) of a workgroup. first[] is an array of its own, so that the search reads two lines of the
+// arguments and not one per group (each a trip to memory: 30 us of the backbone's step).
+template <int N>
+__device__ __forceinline__ int place_of(const int (&first)[N], int blk) {
   int k = 0;
-  while (k + 1 < its.n && blk >= its.it[k + 1].first) ++k;
+  while (k + 1 < N && blk >= first[k + 1]) ++k;
   return k;
 }
-__device__ __forceinline__ int group_of(const NsGroups& gs, int blk) {
-  int k = 0;
-  while (k + 1 < gs.n && blk >= gs.g[k + 1].first) ++k;
-  return k;
+
+// A launch gives group g n = per matrix x count workgroups, rounded up to a multiple of 8, and XCD x (which runs
+// the workgroups i % 8 == x) the x-th eighth of them in order: neighbouring tiles of a matrix share operands,
+// and an XCD finds them in its own 4 MiB L2. Spread over the XCDs, every tile's operands came from beyond
+// the L2s (8 TB/s over the chip, the bound of every product). -1: past the end.
+__device__ __forceinline__ int xcd_local(int b, int n) {
+  const int chunk = (n + 7) >> 3, i = (b & 7) * chunk + (b >> 3);
+  return i < n && (b >> 3) < chunk ? i : -1;
 }
 
 // Sum of squares of one chunk of a matrix, in f64 (squares of every f32 stay in range). STEP: the momentum
@@ -128,10 +157,10 @@ __device__ __forceinline__ int group_of(const NsGroups& gs, int blk) {
 template <typename T, bool STEP>
 __global__ __launch_bounds__(kNormThreads) void ns_norm_kernel(NsGroups gs, NsItems its, float mu, int nesterov) {
   __shared__ double red[kNormThreads / 64];
-  const int k = item_of(its, blockIdx.x);
+  const int k = place_of(its.first, blockIdx.x);
   const NsItem& it = its.it[k];
   const NsGroup& g = gs.g[it.group];
-  const int local = static_cast<int>(blockIdx.x) - it.first, mat = local / g.chunks, chunk = local - mat * g.chunks;
+  const int local = static_cast<int>(blockIdx.x) - its.first[k], mat = local / g.chunks, chunk = local - mat * g.chunks;
   const long long total = static_cast<long long>(g.m) * g.n;
   const long long per = ((total + g.chunks - 1) / g.chunks + 3) & ~3LL;
   const long long e1 = min(total, per * (chunk + 1));
@@ -170,17 +199,32 @@ __global__ __launch_bounds__(kNormThreads) void ns_norm_kernel(NsGroups gs, NsIt
   }
 }
 
+// What takes an update's value to X0's: ldexpf(w f, e), kScale 2^small / (norm + eps) as a factor in [0.5, 1)
+// and a power of two, so that no f32 product leaves the range for any norm.
+struct NsScale {
+  float f;
+  int e, small;
+};
+__device__ __forceinline__ NsScale scale_of(double squares, float eps) {
+  const double norm = sqrt(squares), all = norm + static_cast<double>(eps), part = norm / all;
+  NsScale s;
+  s.small = part > 0.0 ? max(0, -ilogb(part) - 1) : 0;
+  s.f = static_cast<float>(frexp(static_cast<double>(kScale) / all, &s.e));
+  s.e += s.small;
+  return s;
+}
+
 // X0 of one 64 x 64 tile: the (update's) values over their norm, transposed where the matrix is tall, as
 // f16 pairs, zeros in the padding.
 template <typename T, bool STEP>
 __global__ __launch_bounds__(256) void ns_load_kernel(NsGroups gs, NsItems its, float mu, int nesterov, float eps) {
   __shared__ float tile[64][65];
   __shared__ double red[4];
-  const int k = item_of(its, blockIdx.x);
+  const int k = place_of(its.first, blockIdx.x);
   const NsItem& it = its.it[k];
   const NsGroup& g = gs.g[it.group];
   const int tj = g.np / 64, per = (g.mp / 64) * tj;
-  const int local = static_cast<int>(blockIdx.x) - it.first, mat = local / per, t = local - mat * per;
+  const int local = static_cast<int>(blockIdx.x) - its.first[k], mat = local / per, t = local - mat * per;
   const int i0 = (t / tj) * 64, j0 = (t % tj) * 64;
   const long long row = g.target + it.index + mat;
   const double* sums = reinterpret_cast<const double*>(gs.ws + gs.sums) + row * kMaxChunks;
@@ -202,34 +246,30 @@ __global__ __launch_bounds__(256) void ns_load_kernel(NsGroups gs, NsItems its, 
   for (int m = 1; m < 64; m <<= 1) s += __shfl_xor(s, m);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
-  const double norm = sqrt(((red[0] + red[1]) + red[2]) + red[3]);
-  const double part = norm / (norm + static_cast<double>(eps));
-  const int small = part > 0.0 ? max(0, -ilogb(part) - 1) : 0;
-  const double inv = scalbn(static_cast<double>(kScale) / (norm + static_cast<double>(eps)), small);
+  const NsScale sc = scale_of(((red[0] + red[1]) + red[2]) + red[3], eps);
 #pragma unroll
   for (int u = 0; u < 16; ++u) {
     float w = v[u];
     if constexpr (STEP) w = nesterov ? fmaf(mu, o[u], v[u]) : o[u];
     const bool in = r0 + lr + 4 * u < rows && c0 + lc < cols;
-    tile[lr + 4 * u][lc] = in ? static_cast<float>(static_cast<double>(w) * inv) : 0.f;
+    tile[lr + 4 * u][lc] = in ? ldexpf(w * sc.f, sc.e) : 0.f;
   }
   __syncthreads();
-  _Float16* hi = plane_of(gs, g, kX0, it.index + mat);
-  _Float16* lo = hi + static_cast<long long>(g.mp) * g.np;
+  _Float16* dst = pairs_of(gs, g, kX0, it.index + mat);
   typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
   const int pj = 2 * (threadIdx.x & 31), pi = threadIdx.x >> 5;
 #pragma unroll
   for (int u = 0; u < 8; ++u) {
     const int i = pi + 8 * u;
     const Pair a = split_pair(g.tall ? tile[pj][i] : tile[i][pj]), b = split_pair(g.tall ? tile[pj + 1][i] : tile[i][pj + 1]);
-    const long long at = static_cast<long long>(i0 + i) * g.np + j0 + pj;
-    *reinterpret_cast<f16x2*>(hi + at) = f16x2{a.hi, b.hi};
-    *reinterpret_cast<f16x2*>(lo + at) = f16x2{a.lo, b.lo};
+    const long long at = at_pair(i0 + i, j0 + pj, g.np);
+    *reinterpret_cast<f16x2*>(dst + at) = f16x2{a.hi, b.hi};
+    *reinterpret_cast<f16x2*>(dst + at + kLo) = f16x2{a.lo, b.lo};
   }
   if (t == 0 && threadIdx.x == 0) {
     NsTarget* tg = reinterpret_cast<NsTarget*>(gs.ws + gs.targets) + row;
     *tg = NsTarget{STEP ? static_cast<void*>(it.p + mat * it.sb) : static_cast<void*>(reinterpret_cast<T*>(it.p) + mat * it.ob),
-                   it.rate, it.keep, small};
+                   it.rate, it.keep, sc.small};
   }
 }
 
@@ -257,34 +297,53 @@ struct NsJobs {
 
 enum NsMode { kSym = 0, kApply = 1, kWide = 2, kTall = 3 };
 
-// LDS image of a 32-k stage. Operands with k along their rows (NT): [row][32 k], 64-B rows, 16-B chunk c of
-// row r at c ^ ((r >> 2) & 3). X as the right operand of Q X has k down its rows: [k][T columns], chunk c
-// of row r XORed so that the four k rows of one transposed read start on different banks.
-__device__ __forceinline__ constexpr int nt_swz(int r) { return (r >> 2) & 3; }
-template <int T>
-__device__ __forceinline__ constexpr int kx_swz(int r) {
-  return T == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : ((r >> 1) & 1) << 2;
-}
+// LDS image of a 32-k stage, rows of hi and lo as in memory, 16-B chunk c of row r at c ^ swizzle(r).
+// Operands with k along their rows (NT): 128-B rows, and 16 lanes read one chunk of 16 consecutive rows. X as
+// the right operand of Q X has k down its rows (4 T bytes each), and a transposed read takes 64 B of 4
+// consecutive rows.
+__device__ __forceinline__ constexpr int nt_swz(int r) { return (r >> 1) & 7; }
+__device__ __forceinline__ constexpr int kx_swz(int r) { return (r & 3) << 2; }
 
-constexpr int kStages = 3;
-constexpr int stage_bytes(int T) { return 2 * 2 * T * 64; }  // two operands of two planes
+#ifndef NS64
+#define NS64 4
+#endif
+#ifndef NS128
+#define NS128 2
+#endif
+constexpr int ring_of(int T) { return T == 128 ? NS128 : NS64; }
+constexpr int stage_bytes(int T) { return 2 * T * 128; }
+
+// Waits until at most min(later, MOST) stages of PER loads each are in flight, then for the other waves.
+template <int PER, int MOST>
+__device__ __forceinline__ void stage_wait(int later) {
+  if constexpr (MOST > 0) {
+    if (later < MOST) {
+      stage_wait<PER, MOST - 1>(later);
+      return;
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PER * MOST) : "memory");
+}
 
 // T x T output tile, 4 waves of (T / 2) x (T / 2). Three LDS stages filled by LDS-DMA two stages ahead of
 // the products (one barrier a stage); 3 MFMAs per 32 x 32 x 16 block.
 template <int T, int MODE, int OUT>
-__global__ __launch_bounds__(256, 1) void ns_product_kernel(NsGroups gs, NsJobs js) {
-  constexpr int MI = T / 64, kPieces = T / 32;  // 1-KiB DMA pieces per operand plane and wave
-  constexpr int kPlane = T * 64;                // bytes of one operand plane of a stage
+__global__ __launch_bounds__(256, 160 * 1024 / (ring_of(T) * stage_bytes(T))) void ns_product_kernel(NsGroups gs, NsJobs js) {
+  constexpr int MI = T / 64, kPieces = T / 32;  // 1-KiB DMA pieces per operand and wave
+  constexpr int kOperand = T * 128;             // bytes of one operand of a stage
+  constexpr int kStages = ring_of(T);
   constexpr bool KX = MODE != kSym;             // the right operand's k runs down its rows
   extern __shared__ __attribute__((aligned(16))) unsigned char sm[];
   const unsigned S0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)sm));
   const int lane = threadIdx.x & 63, wave = bf16l::wave_id(), j = lane & 31, h = lane >> 5;
-  const NsGroup& g = gs.g[group_of(gs, blockIdx.x)];
-  int local = static_cast<int>(blockIdx.x) - g.first;
+  const int gi = place_of(gs.first, blockIdx.x);
+  const NsGroup& g = gs.g[gi];
   const int nt = (g.mp + T - 1) / T, nc = KX ? (g.np + T - 1) / T : nt;
   const int tiles = KX ? nt * nc : nt * (nt + 1) / 2;
   const int splits = MODE == kSym && js.partial ? g.split : 1;
   const int per = tiles * splits * (MODE == kSym ? js.n : 1);
+  int local = xcd_local(static_cast<int>(blockIdx.x) - gs.first[gi], per * g.count);
+  if (local < 0) return;
   const int mat = local / per;
   local -= mat * per;
   const int jb = MODE == kSym ? local / (tiles * splits) : 0;
@@ -302,38 +361,34 @@ __global__ __launch_bounds__(256, 1) void ns_product_kernel(NsGroups gs, NsJobs 
   if (MODE == kSym && job.l <= kX1) job.inv = ldexpf(job.inv, -2 * x_shift(target_of(gs, g, mat), job.grown));
   const int K = MODE == kSym && job.l <= kX1 ? g.np : g.mp;
   const int i0 = ti * T, c0 = tc * T;
-  const _Float16* L = plane_of(gs, g, job.l, mat);
-  const _Float16* R = plane_of(gs, g, job.r, mat);
-  const unsigned lbytes = static_cast<unsigned>(2LL * g.mp * K);  // one plane
-  const unsigned rbytes = KX ? static_cast<unsigned>(2LL * g.mp * g.np) : lbytes;
+  const _Float16* L = pairs_of(gs, g, job.l, mat);
+  const _Float16* R = pairs_of(gs, g, job.r, mat);
+  const unsigned lbytes = static_cast<unsigned>(4LL * g.mp * K), rbytes = KX ? static_cast<unsigned>(x_bytes(g)) : lbytes;
   const int nst_all = K / 32;
   const int st0 = nst_all * z / splits, nst = nst_all * (z + 1) / splits - st0;
 
-  const int pl = wave >> 1, half = wave & 1;
-  const rsrc_t rl = make_rsrc(reinterpret_cast<const unsigned char*>(L) + static_cast<long long>(pl) * lbytes, lbytes);
-  const rsrc_t rr = make_rsrc(reinterpret_cast<const unsigned char*>(R) + static_cast<long long>(pl) * rbytes, rbytes);
+  const rsrc_t rl = make_rsrc(L, lbytes), rr = make_rsrc(R, rbytes);
   unsigned vol[kPieces], vor[kPieces];
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
-    const int q = kPieces * half + i, r = 16 * q + (lane >> 2), lc = (lane & 3) ^ nt_swz(r);
-    vol[i] = i0 + r < g.mp ? static_cast<unsigned>((static_cast<long long>(i0 + r) * K + 8 * lc) * 2) : kOOB;
+    const int q = kPieces * wave + i, r = 8 * q + (lane >> 3), ch = (lane & 7) ^ nt_swz(r);
+    vol[i] = i0 + r < g.mp ? static_cast<unsigned>(static_cast<long long>(i0 + r) * K * 4 + 16 * ch) : kOOB;
     if constexpr (!KX) {
-      vor[i] = c0 + r < g.mp ? static_cast<unsigned>((static_cast<long long>(c0 + r) * K + 8 * lc) * 2) : kOOB;
+      vor[i] = c0 + r < g.mp ? static_cast<unsigned>(static_cast<long long>(c0 + r) * K * 4 + 16 * ch) : kOOB;
     } else {
-      constexpr int kCh = T / 8, kRows = 64 / kCh;  // 16-B chunks a row, k rows a piece
-      const int kr = kRows * q + lane / kCh, ch = (lane % kCh) ^ kx_swz<T>(kr);
-      vor[i] = c0 + 8 * ch < g.np ? static_cast<unsigned>((static_cast<long long>(kr) * g.np + c0 + 8 * ch) * 2) : kOOB;
+      constexpr int kCh = T / 4, kRows = 64 / kCh;  // 16-B chunks a row, k rows a piece
+      const int kr = kRows * q + lane / kCh, cx = (lane % kCh) ^ kx_swz(kr);
+      vor[i] = c0 + 4 * cx < g.np ? static_cast<unsigned>((static_cast<long long>(kr) * g.np + c0) * 4 + 16 * cx) : kOOB;
     }
   }
   auto issue = [&](int st) __attribute__((always_inline)) {
-    const unsigned base = S0 + static_cast<unsigned>((st % kStages) * stage_bytes(T)) +
-                          static_cast<unsigned>(pl * kPlane + kPieces * half * 1024);
-    const unsigned sl = static_cast<unsigned>(st0 + st) * 64u;
-    const unsigned sr = KX ? static_cast<unsigned>(st0 + st) * 64u * static_cast<unsigned>(g.np) : sl;
+    const unsigned base = S0 + static_cast<unsigned>((st % kStages) * stage_bytes(T) + kPieces * wave * 1024);
+    const unsigned sl = static_cast<unsigned>(st0 + st) * 128u;
+    const unsigned sr = KX ? static_cast<unsigned>(st0 + st) * 128u * static_cast<unsigned>(g.np) : sl;
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) dma16(rl, base + static_cast<unsigned>(i * 1024), vol[i], sl);
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) dma16(rr, base + static_cast<unsigned>(2 * kPlane + i * 1024), vor[i], sr);
+    for (int i = 0; i < kPieces; ++i) dma16(rr, base + static_cast<unsigned>(kOperand + i * 1024), vor[i], sr);
   };
 
   const int wi = (wave & 1) * (T / 2), wc = (wave >> 1) * (T / 2);
@@ -346,18 +401,12 @@ __global__ __launch_bounds__(256, 1) void ns_product_kernel(NsGroups gs, NsJobs 
 #pragma unroll
     for (int b = 0; b < MI; ++b) acc[a][b] = cross[a][b] = zero16();
 
-  if (nst > 0) issue(0);
-  if (nst > 1) issue(1);
+  for (int st = 0; st < kStages - 1 && st < nst; ++st) issue(st);
   for (int st = 0; st < nst; ++st) {
-    // this stage has landed (the next one's 2 kPieces loads of this wave may be in flight), and every
-    // read of the stage before it has returned
-    if (st + 1 < nst) {
-      if constexpr (T == 128) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      else asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    }
-    if (st + 2 < nst) issue(st + 2);  // into the stage that every wave has read before this barrier
+    // this stage has landed (what was issued after it may be in flight), and every read of the stage before
+    // it has returned
+    stage_wait<2 * kPieces, kStages - 2>(nst - 1 - st);
+    if (st + kStages - 1 < nst) issue(st + kStages - 1);  // into the stage that every wave has read before this barrier
     const unsigned sb = S0 + static_cast<unsigned>((st % kStages) * stage_bytes(T));
     f16x8 lf[2][MI][2], rf[2][MI][2];
     auto read_step = [&](int ks) __attribute__((always_inline)) {
@@ -367,18 +416,17 @@ __global__ __launch_bounds__(256, 1) void ns_product_kernel(NsGroups gs, NsJobs 
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           lf[ks][a][t] = *reinterpret_cast<const __attribute__((address_space(3))) f16x8*>(static_cast<uintptr_t>(
-              sb + static_cast<unsigned>(t * kPlane + r * 64 + 16 * ((2 * ks + h) ^ nt_swz(r)))));
+              sb + static_cast<unsigned>(r * 128 + 16 * ((4 * t + 2 * ks + h) ^ nt_swz(r)))));
           if constexpr (!KX) {
             rf[ks][a][t] = *reinterpret_cast<const __attribute__((address_space(3))) f16x8*>(static_cast<uintptr_t>(
-                sb + static_cast<unsigned>((2 + t) * kPlane + c * 64 + 16 * ((2 * ks + h) ^ nt_swz(c)))));
+                sb + static_cast<unsigned>(kOperand + c * 128 + 16 * ((4 * t + 2 * ks + h) ^ nt_swz(c)))));
           } else {
             s16x4 v[2];
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
-              const int kr = 16 * ks + 8 * h + 4 * hf + q4, ch = (wc + 32 * a) / 8 + 2 * (gq & 1) + (p4 >> 1);
+              const int kr = 16 * ks + 8 * h + 4 * hf + q4, ch = (wc + 32 * a) / 4 + 4 * t + 2 * (gq & 1) + (p4 >> 1);
               v[hf] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4*>(
-                  static_cast<uintptr_t>(sb + static_cast<unsigned>((2 + t) * kPlane + kr * (2 * T) +
-                                                                    16 * (ch ^ kx_swz<T>(kr)) + 8 * (p4 & 1)))));
+                  static_cast<uintptr_t>(sb + static_cast<unsigned>(kOperand + kr * (4 * T) + 16 * (ch ^ kx_swz(kr)) + 8 * (p4 & 1)))));
             }
             rf[ks][a][t] = __builtin_bit_cast(f16x8, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
           }
@@ -436,13 +484,12 @@ __global__ __launch_bounds__(256, 1) void ns_product_kernel(NsGroups gs, NsJobs 
         float v[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) v[r] = acc[a][b][r] * job.inv;
-        const long long psz = static_cast<long long>(g.mp) * g.mp;
-        const long long mir = static_cast<long long>(cb + j) * g.mp + ib + 4 * h;  // + 8 q: four rows of column cb + j
+        const long long mir = at_pair(cb + j, ib, g.mp) + 4 * h;  // + 8 q: four rows of column cb + j
         if (job.poly) {
-          const _Float16* A = plane_of(gs, g, kA, mat);
+          const _Float16* A = pairs_of(gs, g, kA, mat);
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const f16x4 ah = *reinterpret_cast<const f16x4*>(A + mir + 8 * q), al = *reinterpret_cast<const f16x4*>(A + psz + mir + 8 * q);
+            const f16x4 ah = *reinterpret_cast<const f16x4*>(A + mir + 8 * q), al = *reinterpret_cast<const f16x4*>(A + mir + 8 * q + kLo);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float x = (static_cast<float>(ah[e]) + static_cast<float>(al[e])) * (1.f / kScale);
@@ -451,34 +498,26 @@ __global__ __launch_bounds__(256, 1) void ns_product_kernel(NsGroups gs, NsJobs 
             }
           }
         }
-        _Float16* hi = plane_of(gs, g, job.out, mat);
+        _Float16* hi = pairs_of(gs, g, job.out, mat);
         Pair p[16];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          p[r] = split_pair(v[r] * job.so);
-          const long long at = static_cast<long long>(ib + acc_row(r, h)) * g.mp + cb + j;
-          hi[at] = p[r].hi;
-          hi[psz + at] = p[r].lo;
-        }
+        for (int r = 0; r < 16; ++r) p[r] = split_pair(v[r] * job.so);
+        store_block(hi + at_pair(ib, cb, g.mp), p, g.mp, lane);
         if (tc != ti) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             *reinterpret_cast<f16x4*>(hi + mir + 8 * q) = f16x4{p[4 * q].hi, p[4 * q + 1].hi, p[4 * q + 2].hi, p[4 * q + 3].hi};
-            *reinterpret_cast<f16x4*>(hi + psz + mir + 8 * q) = f16x4{p[4 * q].lo, p[4 * q + 1].lo, p[4 * q + 2].lo, p[4 * q + 3].lo};
+            *reinterpret_cast<f16x4*>(hi + mir + 8 * q + kLo) = f16x4{p[4 * q].lo, p[4 * q + 1].lo, p[4 * q + 2].lo, p[4 * q + 3].lo};
           }
         }
       } else if constexpr (MODE == kApply) {
-        _Float16* hi = plane_of(gs, g, job.out, mat);
-        const long long psz = static_cast<long long>(g.mp) * g.np;
+        _Float16* hi = pairs_of(gs, g, job.out, mat);
         const NsTarget& tg = target_of(gs, g, mat);
         const float so = ldexpf(job.inv * job.so, x_shift(tg, job.grows) - x_shift(tg, job.grown));
+        Pair p[16];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const Pair p = split_pair(acc[a][b][r] * so);
-          const long long at = static_cast<long long>(ib + acc_row(r, h)) * g.np + cb + j;
-          hi[at] = p.hi;
-          hi[psz + at] = p.lo;
-        }
+        for (int r = 0; r < 16; ++r) p[r] = split_pair(acc[a][b][r] * so);
+        store_block(hi + at_pair(ib, cb, g.np), p, g.np, lane);
       } else {
         const NsTarget tg = target_of(gs, g, mat);
         const int shift = x_shift(tg, job.grown);
@@ -511,9 +550,12 @@ __global__ __launch_bounds__(256, 1) void ns_product_kernel(NsGroups gs, NsJobs 
 // above the diagonal, each wave every fourth split, and stores it with its mirror image.
 __global__ __launch_bounds__(256) void ns_join_kernel(NsGroups gs, float inv, int grown) {
   __shared__ float red[3][16][64];
-  const NsGroup& g = gs.g[group_of(gs, blockIdx.x)];
+  const int gi = place_of(gs.first, blockIdx.x);
+  const NsGroup& g = gs.g[gi];
   const int nb = g.mp / 32, per = nb * (nb + 1) / 2;
-  const int local = static_cast<int>(blockIdx.x) - g.first, mat = local / per;
+  const int local = xcd_local(static_cast<int>(blockIdx.x) - gs.first[gi], per * g.count);
+  if (local < 0) return;
+  const int mat = local / per;
   int blk = local - mat * per, bi = 0;
   while (blk >= nb - bi) blk -= nb - bi, ++bi;
   const int bc = bi + blk, lane = threadIdx.x & 63, wave = bf16l::wave_id(), j = lane & 31, h = lane >> 5;
@@ -535,26 +577,28 @@ __global__ __launch_bounds__(256) void ns_join_kernel(NsGroups gs, float inv, in
   __syncthreads();
   if (wave) return;
   inv = ldexpf(inv, -2 * x_shift(target_of(gs, g, mat), grown));
-  _Float16* hi = plane_of(gs, g, kA, mat);
+  _Float16* hi = pairs_of(gs, g, kA, mat);
   Pair p[16];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    p[r] = split_pair((((v[r] + red[0][r][lane]) + red[1][r][lane]) + red[2][r][lane]) * inv);
-    const long long at = static_cast<long long>(32 * bi + acc_row(r, h)) * g.mp + 32 * bc + j;
-    hi[at] = p[r].hi;
-    hi[psz + at] = p[r].lo;
-  }
+  for (int r = 0; r < 16; ++r) p[r] = split_pair((((v[r] + red[0][r][lane]) + red[1][r][lane]) + red[2][r][lane]) * inv);
+  store_block(hi + at_pair(32 * bi, 32 * bc, g.mp), p, g.mp, lane);
   if (bc != bi) {
-    const long long mir = static_cast<long long>(32 * bc + j) * g.mp + 32 * bi + 4 * h;
+    const long long mir = at_pair(32 * bc + j, 32 * bi, g.mp) + 4 * h;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       *reinterpret_cast<f16x4*>(hi + mir + 8 * q) = f16x4{p[4 * q].hi, p[4 * q + 1].hi, p[4 * q + 2].hi, p[4 * q + 3].hi};
-      *reinterpret_cast<f16x4*>(hi + psz + mir + 8 * q) = f16x4{p[4 * q].lo, p[4 * q + 1].lo, p[4 * q + 2].lo, p[4 * q + 3].lo};
+      *reinterpret_cast<f16x4*>(hi + mir + 8 * q + kLo) = f16x4{p[4 * q].lo, p[4 * q + 1].lo, p[4 * q + 2].lo, p[4 * q + 3].lo};
     }
   }
 }
 
-// ---- host -------------------------------------------------------------------------------------------
+// ---- one workgroup per matrix ---------------------------------------------------------------------------
+
+// Matrices of up to 64 rows and 384 columns (padded): norm, X and all products of one matrix in one
+// workgroup, X and four 64 x 64 matrices in LDS (64 * 384 * 4 + 4 * 16 KiB = 160 KiB). Such a matrix is a
+// chain of some 20 products of well under 1 us each, and a launch each costs 4 to 5 us.
+constexpr int kSmallM = 64, kSmallN = 384, kSmallThreads = 512;
+constexpr int kSmallSquare = 64 * 256;  // bytes of a 64 x 64 matrix of pairs
 
 struct NsPlan {
   int phases[kMaxSteps], nphase;
@@ -562,6 +606,329 @@ struct NsPlan {
   float sp[kMaxSteps], sq[kMaxSteps];  // scales of P and of Q after each step
   int grown[kMaxSteps + 1];            // X before each phase is at most 2^grown times X0
 };
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) f16x8 lds_f16x8;
+typedef __attribute__((address_space(3))) f16x4 lds_f16x4;
+typedef __attribute__((address_space(3))) _Float16 lds_f16;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) float lds_f32;
+template <typename P>
+__device__ __forceinline__ P* lds_ptr(unsigned at) {
+  return reinterpret_cast<P*>(static_cast<uintptr_t>(at));
+}
+
+// LDS rows of pairs (32 hi, 32 lo, ...), pitch a multiple of 256 B; 16-B chunk c of row r at c ^ sm_swz(r):
+// 16 rows of one chunk lie on distinct banks, and so do 64 B of 4 consecutive rows (a transposed read).
+// The lo chunk of hi chunk c is c + 4, at the hi chunk's address ^ 64.
+__device__ __forceinline__ constexpr int sm_swz(int r) { return ((r & 3) << 2) | ((r >> 2) & 3); }
+__device__ __forceinline__ unsigned sm_at(unsigned base, int pitch, int r, int chunk) {
+  return base + static_cast<unsigned>(r * pitch + 16 * (chunk ^ sm_swz(r)));
+}
+__device__ __forceinline__ int chunk_of(int c) { return (c >> 5) * 8 + ((c & 31) >> 3); }  // of column c's hi
+// The 32x32x16 fragment of rows r0 + (lane & 31), k = 16 step + 8 (lane >> 5) .. + 7.
+__device__ __forceinline__ void sm_rows(f16x8 (&f)[2], unsigned base, int pitch, int r0, int step, int lane) {
+  const unsigned at = sm_at(base, pitch, r0 + (lane & 31), (step >> 1) * 8 + 2 * (step & 1) + (lane >> 5));
+  f[0] = *lds_ptr<lds_f16x8>(at);
+  f[1] = *lds_ptr<lds_f16x8>(at ^ 64);
+}
+// The 16x16x32 fragment of rows r0 + (lane & 15), k = 32 step + 8 (lane >> 4) .. + 7.
+__device__ __forceinline__ void sm_rows16(f16x8 (&f)[2], unsigned base, int r0, int step, int lane) {
+  const unsigned at = sm_at(base, 256, r0 + (lane & 15), step * 8 + (lane >> 4));
+  f[0] = *lds_ptr<lds_f16x8>(at);
+  f[1] = *lds_ptr<lds_f16x8>(at ^ 64);
+}
+// sm_rows of columns c0 + (lane & 31), with k down the rows.
+__device__ __forceinline__ void sm_cols(f16x8 (&f)[2], unsigned base, int pitch, int c0, int step, int lane) {
+  const int g = lane >> 4, q = (lane >> 2) & 3, p = lane & 3;
+  s16x4 v[2][2];
+#pragma unroll
+  for (int hf = 0; hf < 2; ++hf) {
+    const int r = 16 * step + 8 * (lane >> 5) + 4 * hf + q;
+    const unsigned at = sm_at(base, pitch, r, (c0 >> 5) * 8 + 2 * (g & 1) + (p >> 1)) + 8 * (p & 1);
+    v[0][hf] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr<lds_s16x4>(at));
+    v[1][hf] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr<lds_s16x4>(at ^ 64));
+  }
+#pragma unroll
+  for (int t = 0; t < 2; ++t) f[t] = __builtin_bit_cast(f16x8, __builtin_shufflevector(v[t][0], v[t][1], 0, 1, 2, 3, 4, 5, 6, 7));
+}
+__device__ __forceinline__ void mma_pairs(f32x16& acc, f32x16& cross, const f16x8 (&l)[2], const f16x8 (&r)[2]) {
+  cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[1], r[0], cross, 0, 0, 0);
+  cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[0], r[1], cross, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[0], r[0], acc, 0, 0, 0);
+}
+// Lane-dependent addresses of one product are formed where they are used: kept for the next one, they spill.
+__device__ __forceinline__ int anew(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// The product L R^T of two symmetric 64 x 64 matrices that commute (so the result is symmetric too) by 8 waves:
+// wave w has rows 16 (w & 3) .. + 15 and columns 32 (w >> 2) .. + 31, as two 16 x 16 blocks (lane: column
+// lane & 15, rows 4 (lane >> 4) .. + 3).
+__device__ __forceinline__ void sm_square(unsigned l, unsigned r, float mul, f32x4 (&v)[2], int wave, int lane) {
+  const int ln = anew(lane);
+  f32x4 acc[2], cross[2];
+#pragma unroll
+  for (int b = 0; b < 2; ++b) acc[b] = cross[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int st = 0; st < 2; ++st) {
+    f16x8 lf[2], rf[2];
+    sm_rows16(lf, l, 16 * (wave & 3), st, ln);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      sm_rows16(rf, r, 32 * (wave >> 2) + 16 * b, st, ln);
+      cross[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lf[1], rf[0], cross[b], 0, 0, 0);
+      cross[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lf[0], rf[1], cross[b], 0, 0, 0);
+      acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lf[0], rf[0], acc[b], 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < 2; ++b) v[b] = (acc[b] + cross[b]) * mul;
+}
+// Where a lane's 4 rows of one column go: the result is symmetric, so they are 4 columns of one row, 8 B.
+__device__ __forceinline__ unsigned sm_mirror(unsigned base, int b, int wave, int lane) {
+  const int row = 32 * (wave >> 2) + 16 * b + (lane & 15), col = 16 * (wave & 3) + 4 * (lane >> 4);
+  return sm_at(base, 256, row, chunk_of(col)) + static_cast<unsigned>(2 * (col & 7));
+}
+__device__ __forceinline__ void sm_put(unsigned base, const f32x4 (&v)[2], int wave, int lane) {
+  const int ln = anew(lane);
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    f16x4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const Pair p = split_pair(v[b][e]);
+      hi[e] = p.hi;
+      lo[e] = p.lo;
+    }
+    const unsigned at = sm_mirror(base, b, wave, ln);
+    *lds_ptr<lds_f16x4>(at) = hi;
+    *lds_ptr<lds_f16x4>(at ^ 64) = lo;
+  }
+}
+
+template <typename T, bool STEP>
+__global__ __launch_bounds__(kSmallThreads, 1) void ns_small_kernel(NsItems its, NsPlan pl, float mu, int nesterov, float eps) {
+  extern __shared__ __attribute__((aligned(256))) unsigned char sm[];
+  const unsigned S0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)sm));
+  const int k = place_of(its.first, blockIdx.x);
+  const NsItem& it = its.it[k];
+  const int mat = static_cast<int>(blockIdx.x) - its.first[k];
+  const int rows = it.rows, cols = it.cols, tall = rows > cols;
+  const int m = tall ? cols : rows, n = tall ? rows : cols, np = (n + 63) & ~63;
+  const int lane = threadIdx.x & 63, wave = bf16l::wave_id(), j = lane & 31, h = lane >> 5;
+  const unsigned MA = S0, MP = S0 + kSmallSquare, MQ = S0 + 2 * kSmallSquare, MT = S0 + 3 * kSmallSquare, X = S0 + 4 * kSmallSquare;
+  const int xp = np * 4;  // pitch of X
+  const T* src = static_cast<const T*>(it.src) + mat * it.sb;
+  float* buf = STEP ? it.buf + mat * it.sb : nullptr;
+
+  // The update (and the momentum) in registers, and its squares in f64. A thread takes runs of 8 values along
+  // X's rows, which are one 16-B chunk of hi and one of lo: row i, columns 8 kc .. + 7.
+  constexpr int kRuns = kSmallM * kSmallN / 8 / kSmallThreads;
+  const int nc = (n + 7) >> 3, runs = m * nc;
+  float v0[kRuns][8];
+  double s = 0.0;
+#pragma unroll
+  for (int q = 0; q < kRuns; ++q) {
+    if (q * kSmallThreads < runs) {
+      const int id = static_cast<int>(threadIdx.x) + q * kSmallThreads, idc = min(id, runs - 1);
+      const int kc = tall ? idc / m : idc % nc, i = tall ? idc % m : idc / nc;
+      const int at = tall ? 8 * kc * cols + i : i * cols + 8 * kc, step = tall ? cols : 1, left = n - 8 * kc;
+      float x[8], o[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int a = at + min(e, left - 1) * step;
+        x[e] = src_at<T>(src, a);
+        if constexpr (STEP) o[e] = buf[a];
+      }
+      pin_batch(x);
+      if constexpr (STEP) pin_batch(o);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool in = id < runs && e < left;
+        float w = x[e];
+        if constexpr (STEP) {
+          const float nb = fmaf(mu, o[e], x[e]);
+          if (in) buf[at + e * step] = nb;
+          w = nesterov ? fmaf(mu, nb, x[e]) : nb;
+        }
+        w = in ? w : 0.f;
+        s = fma(static_cast<double>(w), static_cast<double>(w), s);
+        v0[q][e] = w;
+      }
+    }
+  }
+  // X is zero where no run lies: rows m .. 63, columns 8 nc .. np - 1
+  for (int e = threadIdx.x; e < 64 * np / 4; e += kSmallThreads) *lds_ptr<lds_f16x8>(X + 16 * e) = f16x8{};
+  for (int b = 1; b < 64; b <<= 1) s += __shfl_xor(s, b);
+  double* red = reinterpret_cast<double*>(sm);
+  if (lane == 0) red[wave] = s;
+  __syncthreads();
+  s = 0.0;
+#pragma unroll
+  for (int w = 0; w < kSmallThreads / 64; ++w) s += red[w];
+  const NsScale sc = scale_of(s, eps);
+  const NsTarget tg{nullptr, 0.f, 0.f, sc.small};
+#pragma unroll
+  for (int q = 0; q < kRuns; ++q) {
+    const int id = static_cast<int>(threadIdx.x) + q * kSmallThreads;
+    if (id < runs) {
+      const int kc = tall ? id / m : id % nc, i = tall ? id % m : id / nc;
+      f16x8 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const Pair p = split_pair(ldexpf(v0[q][e] * sc.f, sc.e));
+        hi[e] = p.hi;
+        lo[e] = p.lo;
+      }
+      const unsigned at = sm_at(X, xp, i, chunk_of(8 * kc));
+      *lds_ptr<lds_f16x8>(at) = hi;
+      *lds_ptr<lds_f16x8>(at ^ 64) = lo;
+    }
+  }
+  __syncthreads();
+
+  const int bi = 32 * (wave & 1), bc = 32 * ((wave >> 1) & 1), part = wave >> 2;
+  for (int p = 0, step = 0; p < pl.nphase; ++p) {
+    {  // A = X X^T, a 32 x 32 block and every second 16 k a wave; the halves meet in MT
+      f32x16 acc = zero16(), cross = zero16();
+      for (int st = part; st < np / 16; st += 2) {
+        f16x8 lf[2], rf[2];
+        sm_rows(lf, X, xp, bi, st, lane);
+        sm_rows(rf, X, xp, bc, st, lane);
+        mma_pairs(acc, cross, lf, rf);
+      }
+      lds_f32* sum = lds_ptr<lds_f32>(MT) + (wave & 3) * 1024 + lane;
+      if (part) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum[64 * r] = acc[r] + cross[r];
+      }
+      __syncthreads();
+      if (!part) {
+        const float mul = ldexpf(1.f / kScale, -2 * x_shift(tg, pl.grown[p]));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {  // four rows of a column, stored as the mirror image's four columns
+          f16x4 hi, lo;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const Pair pr = split_pair(((acc[4 * q + e] + cross[4 * q + e]) + sum[64 * (4 * q + e)]) * mul);
+            hi[e] = pr.hi;
+            lo[e] = pr.lo;
+          }
+          const int col = bi + 8 * q + 4 * h;
+          const unsigned at = sm_at(MA, 256, bc + j, chunk_of(col)) + static_cast<unsigned>(2 * (col & 7));
+          *lds_ptr<lds_f16x4>(at) = hi;
+          *lds_ptr<lds_f16x4>(at ^ 64) = lo;
+        }
+      }
+      __syncthreads();
+    }
+    float sq = 0.f;
+    for (int i = 0; i < pl.phases[p]; ++i, ++step) {
+      const float sp = pl.sp[step];
+      const bool more = i + 1 < pl.phases[p];
+      const unsigned P = i == 0 ? MQ : MP;  // the first P is Q
+      f32x4 v[2], vq[2];
+      sm_square(MA, MA, 1.f / (kScale * kScale), v, wave, lane);
+      {
+        const int ln = anew(lane);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const unsigned at = sm_mirror(MA, b, wave, ln);
+          const f16x4 ah = *lds_ptr<lds_f16x4>(at), al = *lds_ptr<lds_f16x4>(at ^ 64);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = (static_cast<float>(ah[e]) + static_cast<float>(al[e])) * (1.f / kScale);
+            v[b][e] = fmaf(pl.c, v[b][e], pl.b * x);
+            if (16 * (wave & 3) + 4 * (ln >> 4) + e == 32 * (wave >> 2) + 16 * b + (ln & 15)) v[b][e] += pl.a;
+            v[b][e] *= sp;
+          }
+        }
+      }
+      sm_put(P, v, wave, lane);
+      __syncthreads();
+      if (more) {  // T = P A
+        sm_square(P, MA, 1.f / sp, v, wave, lane);
+        sm_put(MT, v, wave, lane);
+      }
+      if (i > 0) {  // Q <- P Q, stored once every wave has read Q
+        sm_square(P, MQ, pl.sq[step] / (sp * sq), vq, wave, lane);
+        sq = pl.sq[step];
+      } else {
+        sq = sp;
+      }
+      __syncthreads();
+      if (i > 0) sm_put(MQ, vq, wave, lane);
+      if (more) {  // A <- T P (at the first step P is Q, which no wave stores then)
+        sm_square(MT, P, 1.f / sp, v, wave, lane);
+        sm_put(MA, v, wave, lane);
+      }
+      __syncthreads();
+    }
+    // X <- Q X, 32 columns a wave; a wave reads its columns whole before it writes them
+    const bool last = p + 1 == pl.nphase;
+    const float mul = 1.f / (sq * kScale);
+    for (int c0 = 32 * wave; c0 < np; c0 += 32 * (kSmallThreads / 64)) {
+      f32x16 acc[2], cross[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) acc[b] = cross[b] = zero16();
+      const int ln = anew(lane);
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        f16x8 xf[2], qf[2];
+        sm_cols(xf, X, xp, c0, st, ln);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          sm_rows(qf, MQ, 256, 32 * b, st, ln);
+          if (last && tall) mma_pairs(acc[b], cross[b], xf, qf);  // transposed: lanes along the result's rows
+          else mma_pairs(acc[b], cross[b], qf, xf);
+        }
+      }
+      if (!last) {
+        const float so = ldexpf(mul * kScale, x_shift(tg, pl.grown[p + 1]) - x_shift(tg, pl.grown[p]));
+        // lane: column c0 + j; row 32 b + 4 h + row_of(r), whose swizzle is a constant of r ^ h
+        const int chunk = chunk_of(c0) + (j >> 3);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const unsigned at = X + static_cast<unsigned>((32 * b + 4 * h) * xp + 2 * (j & 7));
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const Pair pr = split_pair((acc[b][r] + cross[b][r]) * so);
+            const unsigned o = at + static_cast<unsigned>(row_of(r) * xp + 16 * (chunk ^ h ^ sm_swz(row_of(r))));
+            *lds_ptr<lds_f16>(o) = pr.hi;
+            *lds_ptr<lds_f16>(o ^ 64) = pr.lo;
+          }
+        }
+        continue;
+      }
+      T* out = STEP ? nullptr : reinterpret_cast<T*>(it.p) + mat * it.ob;
+      const int shift = x_shift(tg, pl.grown[p]);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int r0 = tall ? c0 : 32 * b, col = (tall ? 32 * b : c0) + j;
+        if (col >= cols) continue;
+        float old[16];
+        if constexpr (STEP) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) old[r] = it.p[min(r0 + acc_row(r, h), rows - 1) * cols + col];
+          pin_batch(old);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int row = r0 + acc_row(r, h);
+          if (row >= rows) continue;
+          const float v = ldexpf((acc[b][r] + cross[b][r]) * mul, -shift);
+          if constexpr (STEP) it.p[row * cols + col] = fmaf(-it.rate, v, it.keep * old[r]);
+          else out[row * cols + col] = static_cast<T>(v);
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ---- host -------------------------------------------------------------------------------------------
 
 float scale_for(double most) {  // the largest power of two up to kScale that keeps `most` below 2^15
   float s = kScale;
@@ -583,7 +950,7 @@ int ns_plan(NsPlan& pl, int steps, float a, float b, float c) {
     pl.phases[p] = (left + pl.nphase - p - 1) / (pl.nphase - p);
     left -= pl.phases[p];
   }
-  constexpr int kGrid = 2048;
+  constexpr int kGrid = 256;  // between two points a map of slope 4 and curvature 50 rises by 1e-4
   double most = 1.001, factor = 1.0;
   for (int p = 0, st = 0; p < pl.nphase; ++p) {
     std::vector<double> s(kGrid + 1), q(kGrid + 1, 1.0);
@@ -697,9 +1064,10 @@ int ns_check(int rows, int cols) {
 template <typename F>
 long long ns_grid(NsGroups& gs, F per) {
   long long blocks = 0;
+  for (int k = gs.n; k < kMaxGroups; ++k) gs.first[k] = 0x7fffffff;
   for (int k = 0; k < gs.n; ++k) {
-    gs.g[k].first = static_cast<int>(blocks < (1LL << 30) ? blocks : (1LL << 30));
-    blocks += per(gs.g[k]) * gs.g[k].count;
+    gs.first[k] = static_cast<int>(blocks < (1LL << 30) ? blocks : (1LL << 30));
+    blocks += (per(gs.g[k]) * gs.g[k].count + 7) / 8 * 8;
   }
   return blocks;
 }
@@ -717,7 +1085,7 @@ int ns_launch(NsGroups gs, const NsJobs& js, hipStream_t st) {
   });
   if (blocks == 0) return PROTOSEG_OK;
   if (int e = ns_blocks_ok(blocks)) return e;
-  constexpr size_t lds = kStages * stage_bytes(T);
+  constexpr size_t lds = static_cast<size_t>(ring_of(T)) * stage_bytes(T);
   if (int e = ensure_lds<ns_product_kernel<T, MODE, OUT>, lds>()) return e;
   KernelTimer t("ns_product_kernel", st);
   hipLaunchKernelGGL((ns_product_kernel<T, MODE, OUT>), dim3(static_cast<unsigned>(blocks)), dim3(256), lds, st, gs, js);
@@ -732,7 +1100,7 @@ int ns_products(NsGroups gs, const NsPlan& pl, hipStream_t st) {
     NsJobs js{};
     for (const NsJob& j : jobs) js.j[js.n++] = j;
     js.a = pl.a, js.b = pl.b, js.c = pl.c, js.partial = partial;
-    return ns_launch<T, kSym, kOutF32>(gs, js, st);
+    return js.j[0].l <= kX1 ? ns_launch<T, kSym, kOutF32>(gs, js, st) : ns_launch<64, kSym, kOutF32>(gs, js, st);
   };
   bool split = false;
   for (int k = 0; k < gs.n; ++k) split = split || gs.g[k].split > 1;
@@ -795,6 +1163,37 @@ int ns_products(const NsGroups& gs, const NsPlan& pl, hipStream_t st) {
   return tiles >= kBigTiles ? ns_products<128, OUT>(gs, pl, st) : ns_products<64, OUT>(gs, pl, st);
 }
 
+// Beside larger matrices a small one is nearly free in their launches; the kernel of its own is for calls
+// that have no others.
+bool ns_is_small(int rows, int cols) {
+  const int m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
+  return m <= kSmallM && pad_of(n) <= kSmallN;
+}
+
+template <typename T, bool STEP>
+int ns_small(const std::vector<NsItem>& items, const NsPlan& pl, float mu, int nesterov, float eps, hipStream_t st) {
+  for (size_t i0 = 0; i0 < items.size(); i0 += kMaxItems) {
+    NsItems its{};
+    long long blocks = 0;
+    int n = 0;
+    for (int k = 0; k < kMaxItems; ++k) its.first[k] = 0x7fffffff;
+    for (size_t i = i0; i < items.size() && i < i0 + kMaxItems; ++i) {
+      its.first[its.n] = static_cast<int>(blocks);
+      its.it[its.n++] = items[i];
+      blocks += items[i].count;
+      if (int e = ns_blocks_ok(blocks)) return e;
+      const int l = items[i].rows > items[i].cols ? items[i].rows : items[i].cols;
+      n = pad_of(l) > n ? pad_of(l) : n;
+    }
+    if (int e = ensure_lds<ns_small_kernel<T, STEP>>()) return e;
+    KernelTimer t("ns_small_kernel", st);
+    hipLaunchKernelGGL((ns_small_kernel<T, STEP>), dim3(static_cast<unsigned>(blocks)), dim3(kSmallThreads),
+                       4 * kSmallSquare + static_cast<size_t>(n) * 4 * kSmallM, st, its, pl, mu, nesterov, eps);
+    if (int e = check_launch("ns_small_kernel")) return e;
+  }
+  return PROTOSEG_OK;
+}
+
 // Sums of squares and X0 of all items, kMaxItems a launch.
 template <typename T, bool STEP>
 int ns_load(const NsGroups& gs, const std::vector<NsItem>& items, float mu, int nesterov, float eps, hipStream_t st) {
@@ -802,10 +1201,11 @@ int ns_load(const NsGroups& gs, const std::vector<NsItem>& items, float mu, int 
     for (size_t i0 = 0; i0 < items.size(); i0 += kMaxItems) {
       NsItems its{};
       long long blocks = 0;
+      for (int k = 0; k < kMaxItems; ++k) its.first[k] = 0x7fffffff;
       for (size_t i = i0; i < items.size() && i < i0 + kMaxItems; ++i) {
         NsItem it = items[i];
         const NsGroup& g = gs.g[it.group];
-        it.first = static_cast<int>(blocks);
+        its.first[its.n] = static_cast<int>(blocks);
         blocks += static_cast<long long>(it.count) * (pass ? static_cast<long long>(g.mp / 64) * (g.np / 64) : g.chunks);
         if (int e = ns_blocks_ok(blocks)) return e;
         its.it[its.n++] = it;
@@ -828,7 +1228,7 @@ using namespace protoseg;
 extern "C" size_t protoseg_orthogonalize_workspace_size(int count, int rows, int cols) {
   if (count <= 0 || rows <= 0 || cols <= 0 || ns_check(rows, cols) != PROTOSEG_OK) return 0;
   NsGroups gs;
-  return ns_layout(gs, {NsMatrix{rows, cols, count}}, nullptr, nullptr);
+  return ns_is_small(rows, cols) ? 0 : ns_layout(gs, {NsMatrix{rows, cols, count}}, nullptr, nullptr);
 }
 
 extern "C" int protoseg_orthogonalize(const void* g, int dtype, int count, int rows, int cols, int64_t stride, int steps, float a,
@@ -846,13 +1246,15 @@ extern "C" int protoseg_orthogonalize(const void* g, int dtype, int count, int r
   if (!g || !out) return fail(PROTOSEG_ERR_INVALID, "orthogonalize: matrices and result must be non-null");
   if (count > 1 && stride < size) return fail(PROTOSEG_ERR_INVALID, "orthogonalize: matrices %lld elements apart overlap", static_cast<long long>(stride));
   NsGroups gs;
-  const size_t need = ns_layout(gs, {NsMatrix{rows, cols, count}}, nullptr, nullptr);
-  if (!workspace || workspace_bytes < need)
+  const bool is_small = ns_is_small(rows, cols);
+  const size_t need = is_small ? 0 : ns_layout(gs, {NsMatrix{rows, cols, count}}, nullptr, nullptr);
+  if (need && (!workspace || workspace_bytes < need))
     return fail(PROTOSEG_ERR_INVALID, "orthogonalize workspace %zu bytes, needs %zu", workspace ? workspace_bytes : 0, need);
   gs.ws = static_cast<unsigned char*>(workspace);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const std::vector<NsItem> items{NsItem{g, static_cast<float*>(out), nullptr, stride, size, count, 0, 0, 0, 0.f, 0.f}};
+  const std::vector<NsItem> items{NsItem{g, static_cast<float*>(out), nullptr, stride, size, count, rows, cols, 0, 0, 0.f, 0.f}};
   auto go = [&](auto tag, auto kind) -> int {
+    if (is_small) return ns_small<decltype(tag), false>(items, pl, 0.f, 0, eps, st);
     if (int e = ns_load<decltype(tag), false>(gs, items, 0.f, 0, eps, st)) return e;
     return ns_products<decltype(kind)::value>(gs, pl, st);
   };
@@ -863,15 +1265,19 @@ extern "C" int protoseg_orthogonalize(const void* g, int dtype, int count, int r
 
 namespace {
 // A call's matrices in runs of at most kMaxGroups shapes (one launch covers a run).
-struct MuonRun {
+struct MuonRun {  // none where all matrices are small (ns_small_kernel)
   std::vector<NsMatrix> mats;
   std::vector<int> from;  // tensor of the call
 };
 int muon_runs(std::vector<MuonRun>& runs, int n, const int32_t* rows, const int32_t* cols) {
   std::vector<std::pair<int, int>> shapes;
+  bool all_small = true;
   for (int i = 0; i < n; ++i) {
     if (int e = ns_check(rows[i], cols[i])) return e;
-    if (rows[i] == 0 || cols[i] == 0) continue;
+    all_small = all_small && ns_is_small(rows[i], cols[i]);
+  }
+  for (int i = 0; i < n; ++i) {
+    if (rows[i] == 0 || cols[i] == 0 || all_small) continue;
     size_t k = 0;
     while (k < shapes.size() && shapes[k] != std::make_pair(rows[i], cols[i])) ++k;
     if (k == shapes.size()) shapes.emplace_back(rows[i], cols[i]);
@@ -909,9 +1315,10 @@ extern "C" int protoseg_muon_step(int n_tensors, float* const* params, const flo
   std::vector<MuonRun> runs;
   if (int e = muon_runs(runs, n_tensors, rows, cols)) return e;
   size_t need = 0;
+  for (int i = 0; i < n_tensors; ++i)
+    if (rows[i] && cols[i] && (!params[i] || !grads[i] || !momentum_bufs[i]))
+      return fail(PROTOSEG_ERR_INVALID, "muon tensor %d: null pointer", i);
   for (const MuonRun& r : runs) {
-    for (int i : r.from)
-      if (!params[i] || !grads[i] || !momentum_bufs[i]) return fail(PROTOSEG_ERR_INVALID, "muon tensor %d: null pointer", i);
     NsGroups gs;
     const size_t n = ns_layout(gs, r.mats, nullptr, nullptr);
     need = n > need ? n : need;
@@ -919,21 +1326,25 @@ extern "C" int protoseg_muon_step(int n_tensors, float* const* params, const flo
   if (need && (!workspace || workspace_bytes < need))
     return fail(PROTOSEG_ERR_INVALID, "muon workspace %zu bytes, needs %zu", workspace ? workspace_bytes : 0, need);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  auto item = [&](int i, int group, int index) {
+    const double r = rows[i], q = cols[i];
+    const double scale = scale_kind == 0 ? sqrt(r > q ? r / q : 1.0) : 0.2 * sqrt(r > q ? r : q);
+    return NsItem{grads[i], params[i], momentum_bufs[i], 0, 0, 1, rows[i], cols[i], group, index, static_cast<float>(lr * scale),
+                  static_cast<float>(1.0 - static_cast<double>(lr) * weight_decay)};
+  };
+  std::vector<NsItem> items;
   for (const MuonRun& run : runs) {
     NsGroups gs;
     std::vector<int> which, index;
     ns_layout(gs, run.mats, &which, &index);
     gs.ws = static_cast<unsigned char*>(workspace);
-    std::vector<NsItem> items;
-    for (size_t k = 0; k < run.mats.size(); ++k) {
-      const int i = run.from[k];
-      const double r = rows[i], q = cols[i];
-      const double scale = scale_kind == 0 ? sqrt(r > q ? r / q : 1.0) : 0.2 * sqrt(r > q ? r : q);
-      items.push_back(NsItem{grads[i], params[i], momentum_bufs[i], 0, 0, 1, which[k], index[k], 0, static_cast<float>(lr * scale),
-                             static_cast<float>(1.0 - static_cast<double>(lr) * weight_decay)});
-    }
+    items.clear();
+    for (size_t k = 0; k < run.mats.size(); ++k) items.push_back(item(run.from[k], which[k], index[k]));
     if (int e = ns_load<float, true>(gs, items, momentum, nesterov ? 1 : 0, eps, st)) return e;
     if (int e = ns_products<kOutStep>(gs, pl, st)) return e;
   }
-  return PROTOSEG_OK;
+  if (!runs.empty()) return PROTOSEG_OK;
+  for (int i = 0; i < n_tensors; ++i)
+    if (rows[i] && cols[i]) items.push_back(item(i, 0, 0));
+  return ns_small<float, true>(items, pl, momentum, nesterov ? 1 : 0, eps, st);
 }
