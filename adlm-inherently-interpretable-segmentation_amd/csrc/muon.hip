@@ -41,11 +41,13 @@ using bf16l::dma16;
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kPad = 64;
 constexpr int kMaxGroups = 24, kMaxItems = 32, kMaxSteps = 32;
 constexpr float kScale = 1024.f;  // of X, A and T: entries below 16 (checked) stay below 2^14
-constexpr long long kBigTiles = 192;
+constexpr long long kThinTiles = 256;  // ns_thin_kernel's tiles at most: it has one workgroup a CU (22 matrices of 256, 792 tiles: 303 us for 195)
+constexpr long long kApplyTiles = 384;  // from so many 128 x 128 tiles of Q X on, they beat 64 x 64 ones (backbone: 1178 us for 1236)
 constexpr int kNormThreads = 256, kMaxChunks = 256;
 constexpr long long kNormLeast = 16384;  // elements per workgroup of the sums of squares
 
@@ -72,6 +74,7 @@ struct NsGroups {
   NsGroup g[kMaxGroups];
   int first[kMaxGroups];  // first workgroup of each group in this launch (no workgroup's from n on)
   int n;
+  int thin;  // the symmetric products run on ns_thin_kernel
   unsigned char* ws;
   long long targets, sums;  // byte offsets: NsTarget[matrices], double[matrices][kMaxChunks]
 };
@@ -129,6 +132,28 @@ __device__ __forceinline__ void store_block(_Float16* dst, const Pair (&p)[16], 
   }
 }
 
+// The block transposed in place, through 4 KiB of LDS of the wave's own (both sides on distinct banks).
+// (Stored from the registers it came in, 8 B down each column, a block took 4 times the cache lines.)
+__device__ __forceinline__ void mirror_block(Pair (&p)[16], unsigned lds, int lane) {
+  const int j = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    *reinterpret_cast<__attribute__((address_space(3))) unsigned*>(
+        static_cast<uintptr_t>(lds + static_cast<unsigned>(4 * (32 * j + (acc_row(r, h) ^ j))))) =
+        static_cast<unsigned>(__builtin_bit_cast(uint16_t, p[r].hi)) |
+        (static_cast<unsigned>(__builtin_bit_cast(uint16_t, p[r].lo)) << 16);
+  wave_lds_fence();
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int row = acc_row(r, h);
+    const unsigned v = *reinterpret_cast<const __attribute__((address_space(3))) unsigned*>(
+        static_cast<uintptr_t>(lds + static_cast<unsigned>(4 * (32 * row + (j ^ row)))));
+    p[r].hi = __builtin_bit_cast(_Float16, static_cast<uint16_t>(v));
+    p[r].lo = __builtin_bit_cast(_Float16, static_cast<uint16_t>(v >> 16));
+  }
+  wave_lds_fence();
+}
+
 template <typename T>
 __device__ __forceinline__ float src_at(const void* p, long long i) {
   return static_cast<float>(static_cast<const T*>(p)[i]);
@@ -168,7 +193,36 @@ __global__ __launch_bounds__(kNormThreads) void ns_norm_kernel(NsGroups gs, NsIt
   float* buf = STEP ? it.buf + mat * it.sb : nullptr;
   double s = 0.0;
   constexpr int kU = 4;
-  for (long long e = per * chunk + threadIdx.x; e < e1; e += kU * kNormThreads) {
+  typedef T vec4 __attribute__((ext_vector_type(4)));
+  long long e = per * chunk;
+  if (((reinterpret_cast<uintptr_t>(src) & (sizeof(vec4) - 1)) | (reinterpret_cast<uintptr_t>(buf) & 15)) == 0) {
+    for (; e + kU * 4 * kNormThreads <= e1; e += kU * 4 * kNormThreads) {  // 4 elements a load
+      vec4 v[kU];
+      f32x4 o[kU];
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const long long i = e + 4 * (u * kNormThreads + static_cast<int>(threadIdx.x));
+        v[u] = *reinterpret_cast<const vec4*>(src + i);
+        if constexpr (STEP) o[u] = *reinterpret_cast<const f32x4*>(buf + i);
+      }
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float x = static_cast<float>(v[u][c]);
+          float w = x;
+          if constexpr (STEP) {
+            o[u][c] = fmaf(mu, o[u][c], x);
+            w = nesterov ? fmaf(mu, o[u][c], x) : o[u][c];
+          }
+          s = fma(static_cast<double>(w), static_cast<double>(w), s);
+        }
+        if constexpr (STEP)
+          *reinterpret_cast<f32x4*>(buf + e + 4 * (u * kNormThreads + static_cast<int>(threadIdx.x))) = o[u];
+      }
+    }
+  }
+  for (e += threadIdx.x; e < e1; e += kU * kNormThreads) {
     float v[kU], o[kU];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
@@ -304,13 +358,9 @@ enum NsMode { kSym = 0, kApply = 1, kWide = 2, kTall = 3 };
 __device__ __forceinline__ constexpr int nt_swz(int r) { return (r >> 1) & 7; }
 __device__ __forceinline__ constexpr int kx_swz(int r) { return (r & 3) << 2; }
 
-#ifndef NS64
-#define NS64 4
-#endif
-#ifndef NS128
-#define NS128 2
-#endif
-constexpr int ring_of(int T) { return T == 128 ? NS128 : NS64; }
+// Stages of the ring: three workgroups a CU at 64, two at 128. Deeper rings measured slower (5 at 64: +3 %, 4 at
+// 128: +5 %): a workgroup beside another hides more than a stage further ahead.
+constexpr int ring_of(int T) { return T == 128 ? 2 : 3; }
 constexpr int stage_bytes(int T) { return 2 * T * 128; }
 
 // Waits until at most min(later, MOST) stages of PER loads each are in flight, then for the other waves.
@@ -484,18 +534,19 @@ __global__ __launch_bounds__(256, 160 * 1024 / (ring_of(T) * stage_bytes(T))) vo
         float v[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) v[r] = acc[a][b][r] * job.inv;
-        const long long mir = at_pair(cb + j, ib, g.mp) + 4 * h;  // + 8 q: four rows of column cb + j
         if (job.poly) {
-          const _Float16* A = pairs_of(gs, g, kA, mat);
+          const _Float16* A = pairs_of(gs, g, kA, mat) + at_pair(ib, cb, g.mp) + j;
+          _Float16 ah[16], al[16];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const f16x4 ah = *reinterpret_cast<const f16x4*>(A + mir + 8 * q), al = *reinterpret_cast<const f16x4*>(A + mir + 8 * q + kLo);
+          for (int r = 0; r < 16; ++r) {
+            ah[r] = A[static_cast<long long>(acc_row(r, h)) * (2 * g.mp)];
+            al[r] = A[static_cast<long long>(acc_row(r, h)) * (2 * g.mp) + kLo];
+          }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float x = (static_cast<float>(ah[e]) + static_cast<float>(al[e])) * (1.f / kScale);
-              v[4 * q + e] = fmaf(js.c, v[4 * q + e], js.b * x);
-              if (ib + 8 * q + 4 * h + e == cb + j) v[4 * q + e] += js.a;
-            }
+          for (int r = 0; r < 16; ++r) {
+            const float x = (static_cast<float>(ah[r]) + static_cast<float>(al[r])) * (1.f / kScale);
+            v[r] = fmaf(js.c, v[r], js.b * x);
+            if (ib + acc_row(r, h) == cb + j) v[r] += js.a;
           }
         }
         _Float16* hi = pairs_of(gs, g, job.out, mat);
@@ -504,11 +555,8 @@ __global__ __launch_bounds__(256, 160 * 1024 / (ring_of(T) * stage_bytes(T))) vo
         for (int r = 0; r < 16; ++r) p[r] = split_pair(v[r] * job.so);
         store_block(hi + at_pair(ib, cb, g.mp), p, g.mp, lane);
         if (tc != ti) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            *reinterpret_cast<f16x4*>(hi + mir + 8 * q) = f16x4{p[4 * q].hi, p[4 * q + 1].hi, p[4 * q + 2].hi, p[4 * q + 3].hi};
-            *reinterpret_cast<f16x4*>(hi + mir + 8 * q + kLo) = f16x4{p[4 * q].lo, p[4 * q + 1].lo, p[4 * q + 2].lo, p[4 * q + 3].lo};
-          }
+          mirror_block(p, S0 + static_cast<unsigned>((nst % kStages) * stage_bytes(T) + wave * 4096), lane);
+          store_block(hi + at_pair(cb, ib, g.mp), p, g.mp, lane);
         }
       } else if constexpr (MODE == kApply) {
         _Float16* hi = pairs_of(gs, g, job.out, mat);
@@ -544,6 +592,128 @@ __global__ __launch_bounds__(256, 160 * 1024 / (ring_of(T) * stage_bytes(T))) vo
         }
       }
     }
+}
+
+// The symmetric products of few matrices: a 32 x 32 tile a workgroup, whose 4 waves take every fourth 32-k stage
+// (a ring of 4 stages of its own each, no barrier in the loop) and then a quarter of the tile's rows each. A
+// launch of few tiles is a chain of load latencies along k: a quarter of it, and four times the workgroups.
+constexpr int kThinRing = 4, kThinStage = 2 * 32 * 128;
+template <int MOST>
+__device__ __forceinline__ void thin_wait(int later) {  // at most min(later, MOST) stages of 8 loads in flight
+  if constexpr (MOST > 0) {
+    if (later < MOST) {
+      thin_wait<MOST - 1>(later);
+      return;
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(8 * MOST) : "memory");
+}
+__global__ __launch_bounds__(256, 1) void ns_thin_kernel(NsGroups gs, NsJobs js) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char sm[];
+  const unsigned S0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)sm));
+  const int lane = threadIdx.x & 63, wave = bf16l::wave_id(), j = lane & 31, h = lane >> 5;
+  const int gi = place_of(gs.first, blockIdx.x);
+  const NsGroup& g = gs.g[gi];
+  const int nt = g.mp / 32, tiles = nt * (nt + 1) / 2, splits = js.partial ? g.split : 1, per = tiles * splits * js.n;
+  int local = xcd_local(static_cast<int>(blockIdx.x) - gs.first[gi], per * g.count);
+  if (local < 0) return;
+  const int mat = local / per;
+  local -= mat * per;
+  const int jb = local / (tiles * splits);
+  local -= jb * tiles * splits;
+  const int z = local / tiles;
+  int tile = local - z * tiles, ti = 0;
+  while (tile >= nt - ti) tile -= nt - ti, ++ti;
+  const int i0 = 32 * ti, c0 = 32 * (ti + tile);
+  NsJob job = js.j[jb];
+  if (job.l <= kX1) job.inv = ldexpf(job.inv, -2 * x_shift(target_of(gs, g, mat), job.grown));
+  const int K = job.l <= kX1 ? g.np : g.mp, nst_all = K / 32;
+  const int st0 = nst_all * z / splits, nst = nst_all * (z + 1) / splits - st0;
+  const int mine = (nst - wave + 3) / 4;  // stages st0 + wave + 4 t
+  const unsigned bytes = static_cast<unsigned>(4LL * g.mp * K);
+  const rsrc_t rl = make_rsrc(pairs_of(gs, g, job.l, mat), bytes), rr = make_rsrc(pairs_of(gs, g, job.r, mat), bytes);
+  unsigned vol[4], vor[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 8 * i + (lane >> 3), ch = (lane & 7) ^ nt_swz(r);
+    vol[i] = static_cast<unsigned>(static_cast<long long>(i0 + r) * K * 4 + 16 * ch);
+    vor[i] = static_cast<unsigned>(static_cast<long long>(c0 + r) * K * 4 + 16 * ch);
+  }
+  const unsigned W0 = S0 + static_cast<unsigned>(wave * kThinRing * kThinStage);
+  auto issue = [&](int t) __attribute__((always_inline)) {
+    const unsigned base = W0 + static_cast<unsigned>((t % kThinRing) * kThinStage);
+    const unsigned so = static_cast<unsigned>(st0 + wave + 4 * t) * 128u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dma16(rl, base + static_cast<unsigned>(i * 1024), vol[i], so);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dma16(rr, base + static_cast<unsigned>(4096 + i * 1024), vor[i], so);
+  };
+  for (int t = 0; t < kThinRing && t < mine; ++t) issue(t);
+  f32x16 acc = zero16(), cross = zero16();
+  for (int t = 0; t < mine; ++t) {
+    thin_wait<kThinRing - 1>(mine - 1 - t);
+    const unsigned sb = W0 + static_cast<unsigned>((t % kThinRing) * kThinStage);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      f16x8 lf[2], rf[2];
+#pragma unroll
+      for (int t2 = 0; t2 < 2; ++t2) {
+        const unsigned at = sb + static_cast<unsigned>(j * 128 + 16 * ((4 * t2 + 2 * ks + h) ^ nt_swz(j)));
+        lf[t2] = *reinterpret_cast<const __attribute__((address_space(3))) f16x8*>(static_cast<uintptr_t>(at));
+        rf[t2] = *reinterpret_cast<const __attribute__((address_space(3))) f16x8*>(static_cast<uintptr_t>(at + 4096));
+      }
+      cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(lf[1], rf[0], cross, 0, 0, 0);
+      cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(lf[0], rf[1], cross, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(lf[0], rf[0], acc, 0, 0, 0);
+    }
+    if (t + kThinRing < mine) {
+      wave_lds_fence();  // the reads of this place have returned
+      issue(t + kThinRing);
+    }
+  }
+  // this wave's place holds nothing any more: its sums, then everyone's rows 8 wave + 4 h .. + 3 of column j
+  float* mysum = reinterpret_cast<float*>(sm + wave * kThinRing * kThinStage);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) mysum[64 * r + lane] = acc[r] + cross[r];
+  __syncthreads();
+  float v[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    v[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) v[e] += reinterpret_cast<const float*>(sm + w * kThinRing * kThinStage)[64 * (4 * wave + e) + lane];
+  }
+  const int row = i0 + 8 * wave + 4 * h, col = c0 + j;
+  if (js.partial && g.split > 1) {
+    float* dst = reinterpret_cast<float*>(gs.ws + g.part) +
+                 (static_cast<long long>(mat) * g.split + z) * g.mp * g.mp + static_cast<long long>(row) * g.mp + col;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) dst[static_cast<long long>(e) * g.mp] = v[e];
+    return;
+  }
+  const long long at = at_pair(row, col, g.mp), mir = at_pair(col, row, g.mp);
+  const _Float16* A = pairs_of(gs, g, kA, mat);
+  _Float16* out = pairs_of(gs, g, job.out, mat);
+  f16x4 hi, lo;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    v[e] *= job.inv;
+    if (job.poly) {
+      const long long a = at + static_cast<long long>(e) * (2 * g.mp);
+      const float x = (static_cast<float>(A[a]) + static_cast<float>(A[a + kLo])) * (1.f / kScale);
+      v[e] = fmaf(js.c, v[e], js.b * x);
+      if (row + e == col) v[e] += js.a;
+    }
+    const Pair p = split_pair(v[e] * job.so);
+    hi[e] = p.hi;
+    lo[e] = p.lo;
+    out[at + static_cast<long long>(e) * (2 * g.mp)] = p.hi;
+    out[at + static_cast<long long>(e) * (2 * g.mp) + kLo] = p.lo;
+  }
+  if (tile) {
+    *reinterpret_cast<f16x4*>(out + mir) = hi;
+    *reinterpret_cast<f16x4*>(out + mir + kLo) = lo;
+  }
 }
 
 // The partials of a split Gram product joined in a fixed order: a workgroup takes one 32 x 32 block on or
@@ -583,12 +753,8 @@ __global__ __launch_bounds__(256) void ns_join_kernel(NsGroups gs, float inv, in
   for (int r = 0; r < 16; ++r) p[r] = split_pair((((v[r] + red[0][r][lane]) + red[1][r][lane]) + red[2][r][lane]) * inv);
   store_block(hi + at_pair(32 * bi, 32 * bc, g.mp), p, g.mp, lane);
   if (bc != bi) {
-    const long long mir = at_pair(32 * bc + j, 32 * bi, g.mp) + 4 * h;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      *reinterpret_cast<f16x4*>(hi + mir + 8 * q) = f16x4{p[4 * q].hi, p[4 * q + 1].hi, p[4 * q + 2].hi, p[4 * q + 3].hi};
-      *reinterpret_cast<f16x4*>(hi + mir + 8 * q + kLo) = f16x4{p[4 * q].lo, p[4 * q + 1].lo, p[4 * q + 2].lo, p[4 * q + 3].lo};
-    }
+    mirror_block(p, static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)&red[0][0][0])), lane);
+    store_block(hi + at_pair(32 * bc, 32 * bi, g.mp), p, g.mp, lane);
   }
 }
 
@@ -607,7 +773,6 @@ struct NsPlan {
   int grown[kMaxSteps + 1];            // X before each phase is at most 2^grown times X0
 };
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) f16x8 lds_f16x8;
 typedef __attribute__((address_space(3))) f16x4 lds_f16x4;
 typedef __attribute__((address_space(3))) _Float16 lds_f16;
@@ -728,12 +893,14 @@ __global__ __launch_bounds__(kSmallThreads, 1) void ns_small_kernel(NsItems its,
   constexpr int kRuns = kSmallM * kSmallN / 8 / kSmallThreads;
   const int nc = (n + 7) >> 3, runs = m * nc;
   float v0[kRuns][8];
+  int place[kRuns];  // i + 64 kc
   double s = 0.0;
 #pragma unroll
   for (int q = 0; q < kRuns; ++q) {
     if (q * kSmallThreads < runs) {
       const int id = static_cast<int>(threadIdx.x) + q * kSmallThreads, idc = min(id, runs - 1);
       const int kc = tall ? idc / m : idc % nc, i = tall ? idc % m : idc / nc;
+      place[q] = i + 64 * kc;
       const int at = tall ? 8 * kc * cols + i : i * cols + 8 * kc, step = tall ? cols : 1, left = n - 8 * kc;
       float x[8], o[8];
 #pragma unroll
@@ -774,7 +941,7 @@ __global__ __launch_bounds__(kSmallThreads, 1) void ns_small_kernel(NsItems its,
   for (int q = 0; q < kRuns; ++q) {
     const int id = static_cast<int>(threadIdx.x) + q * kSmallThreads;
     if (id < runs) {
-      const int kc = tall ? id / m : id % nc, i = tall ? id % m : id / nc;
+      const int kc = place[q] >> 6, i = place[q] & 63;
       f16x8 hi, lo;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -1019,8 +1186,13 @@ size_t ns_layout(NsGroups& gs, const std::vector<NsMatrix>& mats, std::vector<in
   for (int k = 0; k < gs.n; ++k) gs.g[k] = was.g[order[k]], place[order[k]] = k;
   if (which)
     for (int& w : *which) w = place[w];
-  long long tiles = 0;  // 64 x 64 Gram tiles in all
-  for (int k = 0; k < gs.n; ++k) tiles += static_cast<long long>(gs.g[k].count) * (gs.g[k].mp / 64) * (gs.g[k].mp / 64 + 1) / 2;
+  long long tiles = 0, thin = 0;  // 64 x 64 and 32 x 32 tiles of a symmetric product in all
+  for (int k = 0; k < gs.n; ++k) {
+    const long long nt = gs.g[k].mp / 64;
+    tiles += gs.g[k].count * (nt * (nt + 1) / 2);
+    thin += gs.g[k].count * (nt * (2 * nt + 1));
+  }
+  gs.thin = thin <= kThinTiles;
   long long at = 0, total = 0;
   auto take = [&](long long bytes) {
     const long long o = at;
@@ -1032,8 +1204,8 @@ size_t ns_layout(NsGroups& gs, const std::vector<NsMatrix>& mats, std::vector<in
     // The Gram contraction is split where it is long (a split is at least 8 stages) and the launch has
     // fewer tiles than the chip has places for, or its chain of stages would outlast everything else's.
     const long long stages = g.np / 32;
-    long long split = 384 / (tiles < 1 ? 1 : tiles);
-    const long long chain = (stages + 63) / 64, most = stages / 8;
+    long long split = gs.thin ? 1 : 384 / tiles;
+    const long long chain = gs.thin ? (stages + 255) / 256 : (stages + 63) / 64, most = stages / 8;
     if (split < chain) split = chain;
     if (split > most) split = most;
     if (split > 32) split = 32;
@@ -1075,14 +1247,17 @@ int ns_blocks_ok(long long blocks) {
   return blocks < (1LL << 30) ? PROTOSEG_OK : fail(PROTOSEG_ERR_UNSUPPORTED, "orthogonalize: %lld workgroups", blocks);
 }
 
+template <int MODE>
+long long ns_tiles(const NsGroup& g, const NsJobs& js, int T) {
+  const long long nt = ceil_div(g.mp, T);
+  if (MODE == kSym) return nt * (nt + 1) / 2 * js.n * (js.partial ? g.split : 1);
+  if ((MODE == kWide && g.tall) || (MODE == kTall && !g.tall)) return 0;
+  return nt * ceil_div(g.np, T);
+}
+
 template <int T, int MODE, int OUT>
-int ns_launch(NsGroups gs, const NsJobs& js, hipStream_t st) {
-  const long long blocks = ns_grid(gs, [&](const NsGroup& g) -> long long {
-    const long long nt = ceil_div(g.mp, T);
-    if (MODE == kSym) return nt * (nt + 1) / 2 * js.n * (js.partial ? g.split : 1);
-    if ((MODE == kWide && g.tall) || (MODE == kTall && !g.tall)) return 0;
-    return nt * ceil_div(g.np, T);
-  });
+int ns_launch_tile(NsGroups& gs, const NsJobs& js, hipStream_t st) {
+  const long long blocks = ns_grid(gs, [&](const NsGroup& g) { return ns_tiles<MODE>(g, js, T); });
   if (blocks == 0) return PROTOSEG_OK;
   if (int e = ns_blocks_ok(blocks)) return e;
   constexpr size_t lds = static_cast<size_t>(ring_of(T)) * stage_bytes(T);
@@ -1091,16 +1266,34 @@ int ns_launch(NsGroups gs, const NsJobs& js, hipStream_t st) {
   hipLaunchKernelGGL((ns_product_kernel<T, MODE, OUT>), dim3(static_cast<unsigned>(blocks)), dim3(256), lds, st, gs, js);
   return check_launch("ns_product_kernel");
 }
+int ns_launch_thin(NsGroups& gs, const NsJobs& js, hipStream_t st) {
+  const long long blocks = ns_grid(gs, [&](const NsGroup& g) { return ns_tiles<kSym>(g, js, 32); });
+  constexpr size_t lds = 4 * kThinRing * kThinStage;
+  if (int e = ensure_lds<ns_thin_kernel, lds>()) return e;
+  KernelTimer t("ns_thin_kernel", st);
+  hipLaunchKernelGGL(ns_thin_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), lds, st, gs, js);
+  return check_launch("ns_thin_kernel");
+}
+template <int MODE, int OUT>
+int ns_launch(NsGroups gs, const NsJobs& js, hipStream_t st) {
+  if constexpr (MODE == kSym) {
+    return gs.thin ? ns_launch_thin(gs, js, st) : ns_launch_tile<64, MODE, OUT>(gs, js, st);
+  } else {
+    long long big = 0;
+    for (int k = 0; k < gs.n; ++k) big += ns_tiles<MODE>(gs.g[k], js, 128) * gs.g[k].count;
+    return big >= kApplyTiles ? ns_launch_tile<128, MODE, OUT>(gs, js, st) : ns_launch_tile<64, MODE, OUT>(gs, js, st);
+  }
+}
 
 // All products of a prepared X0, ending in the targets.
-template <int T, int OUT>
-int ns_products(NsGroups gs, const NsPlan& pl, hipStream_t st) {
+template <int OUT>
+int ns_products(const NsGroups& gs, const NsPlan& pl, hipStream_t st) {
   int x = kX0, step = 0;
   auto sym = [&](std::initializer_list<NsJob> jobs, int partial = 0) {
     NsJobs js{};
     for (const NsJob& j : jobs) js.j[js.n++] = j;
     js.a = pl.a, js.b = pl.b, js.c = pl.c, js.partial = partial;
-    return js.j[0].l <= kX1 ? ns_launch<T, kSym, kOutF32>(gs, js, st) : ns_launch<64, kSym, kOutF32>(gs, js, st);
+    return ns_launch<kSym, kOutF32>(gs, js, st);
   };
   bool split = false;
   for (int k = 0; k < gs.n; ++k) split = split || gs.g[k].split > 1;
@@ -1142,25 +1335,15 @@ int ns_products(NsGroups gs, const NsPlan& pl, hipStream_t st) {
     if (p + 1 < pl.nphase) {
       const int xn = x == kX0 ? kX1 : kX0;
       js.j[0] = NsJob{q, x, xn, 0, 1.f / (sq * kScale), kScale, pl.grown[p], pl.grown[p + 1]};
-      if (int e = ns_launch<T, kApply, kOutF32>(gs, js, st)) return e;
+      if (int e = ns_launch<kApply, kOutF32>(gs, js, st)) return e;
       x = xn;
     } else {
       js.j[0] = NsJob{q, x, x, 0, 1.f / (sq * kScale), 1.f, pl.grown[p]};
-      if (int e = ns_launch<T, kWide, OUT>(gs, js, st)) return e;
-      if (int e = ns_launch<T, kTall, OUT>(gs, js, st)) return e;
+      if (int e = ns_launch<kWide, OUT>(gs, js, st)) return e;
+      if (int e = ns_launch<kTall, OUT>(gs, js, st)) return e;
     }
   }
   return PROTOSEG_OK;
-}
-
-template <int OUT>
-int ns_products(const NsGroups& gs, const NsPlan& pl, hipStream_t st) {
-  long long tiles = 0;
-  for (int k = 0; k < gs.n; ++k) {
-    const long long nt = ceil_div(gs.g[k].mp, 128);
-    tiles += nt * (nt + 1) / 2 * gs.g[k].count;
-  }
-  return tiles >= kBigTiles ? ns_products<128, OUT>(gs, pl, st) : ns_products<64, OUT>(gs, pl, st);
 }
 
 // Beside larger matrices a small one is nearly free in their launches; the kernel of its own is for calls
