@@ -26,6 +26,7 @@ import torch.nn.functional as F
 from torch import Tensor
 
 from .distributed import GradientBuckets, world_info
+from .norm import GroupNorm
 
 
 def backbone_params(features, key: str):
@@ -46,15 +47,41 @@ def joint_param_groups(ppnet, lr_features: float = 2.5e-5, lr_add_on_layers: flo
                        lr_prototype_vectors: float = 2.5e-4, weight_decay: float = 5e-4):
     """The joint-phase optimizer groups of module.py:357-382 (defaults: cityscapes_*_imnet.gin
     joint_optimizer_*): backbone 1x / 10x / 20x, add-on layers, prototype vectors (no weight
-    decay). BatchNorm and the last layer get gradients but are not stepped, as in the reference."""
+    decay). BatchNorm and the last layer get gradients but are not stepped, as in the reference; a
+    backbone with group norm (``deeplab`` norm="group") has one group more, its affine parameters at
+    the backbone's learning rate without weight decay."""
     wd = weight_decay
+    gn = group_norm_params(ppnet.features)
+    extra = [{"params": gn, "lr": lr_features, "weight_decay": 0.0}] if gn else []
     return [
         {"params": list(backbone_params(ppnet.features, "1x")), "lr": lr_features, "weight_decay": wd},
         {"params": list(backbone_params(ppnet.features, "10x")), "lr": 10 * lr_features, "weight_decay": wd},
         {"params": list(backbone_params(ppnet.features, "20x")), "lr": 10 * lr_features, "weight_decay": wd},
         {"params": list(ppnet.add_on_layers.parameters()), "lr": lr_add_on_layers, "weight_decay": wd},
         {"params": [ppnet.prototype_vectors], "lr": lr_prototype_vectors},
-    ]
+    ] + extra
+
+
+def group_norm_params(module):
+    """The affine parameters of every ``norm.GroupNorm`` below ``module``."""
+    return [p for m in module.modules() if isinstance(m, GroupNorm) for p in m.parameters()]
+
+
+def muon_param_groups(ppnet, lr_matrices: float = 2e-3, lr_vectors: float = 2.5e-4, weight_decay: float = 5e-4):
+    """The joint phase's parameters (joint_param_groups) split for two optimizers: the matrices
+    (convolution weights of the backbone and the add-on layers, prototype vectors) for
+    ``optim.Muon``, and the rest (biases, group norm) for ``optim.Adam``. Pass both to
+    ``PatchClassificationStep(optimizer=[Muon(...), Adam(...)])``."""
+    matrices, vectors = [], []
+    for group in joint_param_groups(ppnet, weight_decay=weight_decay):
+        for p in group["params"]:
+            (matrices if p.dim() >= 2 else vectors).append((p, group.get("weight_decay", 0.0)))
+
+    def groups(params, lr):
+        return [{"params": [p for p, d in params if d == wd], "lr": lr, "weight_decay": wd}
+                for wd in sorted({d for _, d in params}, reverse=True)]
+
+    return groups(matrices, lr_matrices), groups(vectors, lr_vectors)
 
 
 def _default_resize(labels: Tensor, h: int, w: int) -> Tensor:
@@ -76,6 +103,7 @@ class PatchClassificationStep:
     ``ppnet(image)`` must return ``(logits [B, h, w, K], distances [B, P, h, w])`` or a list of
     such pairs (PPNet.forward with patch_classification). ``target`` is the label map at image
     resolution [B, H, W] (resized here with PIL-nearest semantics) or already at [B, h, w].
+    ``optimizer`` may be a list: each parameter in one of them, all stepped at the boundary.
     ``kld_fn(distances, target_img, class_identity) -> (mean loss, n_pairs)`` and
     ``resize_fn(labels, h, w)`` default to the HIP kernels.
     """
@@ -86,6 +114,7 @@ class PatchClassificationStep:
                  kld_fn: Optional[Callable] = None, resize_fn: Optional[Callable] = None):
         self.ppnet = ppnet
         self.optimizer = optimizer
+        self.optimizers = list(optimizer) if isinstance(optimizer, (list, tuple)) else [optimizer]
         self.loss_weight_crs_ent = loss_weight_crs_ent
         self.loss_weight_kld = loss_weight_kld
         self.loss_weight_l1 = loss_weight_l1
@@ -162,7 +191,8 @@ class PatchClassificationStep:
         if self.iter_steps == 0:
             # in place, as the reference's optimizer.zero_grad() (module.py:122; torch 1.10's
             # default): the gradients stay views into the exchange buckets' buffers
-            self.optimizer.zero_grad(set_to_none=False)
+            for opt in self.optimizers:
+                opt.zero_grad(set_to_none=False)
         boundary = self.iter_steps + 1 == self.iter_size
         if boundary:
             self.buckets.arm()  # the exchange rides on this backward's gradient hooks
@@ -177,7 +207,8 @@ class PatchClassificationStep:
         """The accumulation boundary: gradient exchange (if not already overlapped), optimizer
         and scheduler step (module.py:238-243)."""
         self.buckets.wait()
-        self.optimizer.step()
+        for opt in self.optimizers:
+            opt.step()
         if self.lr_scheduler is not None:
             self.lr_scheduler.step()
         self.iter_steps = 0
