@@ -9,7 +9,8 @@
 // For an m x n matrix that is 3 m^2 n + O(m^3) multiply-adds a phase against 4 m^2 n a step. A's rounding
 // (2^-22 of its norm) can leave a zero eigenvalue slightly negative, and every step multiplies it by a^2:
 // a phase is cut where that could reach 2^-13 (3 steps at a = 3.4445), and the next one starts from a new
-// X X^T, which has no negative eigenvalues. The default five steps run as 3 + 2.
+// X X^T, which has no negative eigenvalues. The default five steps run as 3 + 2, or in shorter phases where
+// the result is to be exact to f32 (ns_exact_longest).
 //
 // Products run on v_mfma_f32_32x32x16_f16 with every operand held as a pair of f16 values, hi + lo of the
 // value times a power of two (22 bits, no overflow: singular values are bounded by the scalar map, checked
@@ -828,48 +829,64 @@ __device__ __forceinline__ int anew(int v) {
   return v;
 }
 
-// The product L R^T of two symmetric 64 x 64 matrices that commute (so the result is symmetric too) by 8 waves:
-// wave w has rows 16 (w & 3) .. + 15 and columns 32 (w >> 2) .. + 31, as two 16 x 16 blocks (lane: column
-// lane & 15, rows 4 (lane >> 4) .. + 3).
+// The product L R^T of two symmetric 64 x 64 matrices that commute, so that it is symmetric too: the 10 blocks of
+// 16 x 16 on and above the diagonal, block w to wave w and blocks 8 and 9 to the first two again. A lane has
+// column lane & 15 and rows 4 (lane >> 4) .. + 3 of a block. Blocks above the diagonal are stored with their
+// mirror images: a result that is symmetric but for its roundings drifts, to twice the error over five steps.
+struct SmBlock {
+  int r0, c0;
+  bool on;
+};
+__device__ __forceinline__ SmBlock sm_block(int wave, int turn) {
+  const int t = wave + 8 * turn, bi = t < 4 ? 0 : t < 7 ? 1 : t < 9 ? 2 : 3, bc = t < 4 ? t : t < 7 ? t - 3 : t < 9 ? t - 5 : 3;
+  return SmBlock{16 * bi, 16 * bc, t < 10};
+}
 __device__ __forceinline__ void sm_square(unsigned l, unsigned r, float mul, f32x4 (&v)[2], int wave, int lane) {
   const int ln = anew(lane);
-  f32x4 acc[2], cross[2];
 #pragma unroll
-  for (int b = 0; b < 2; ++b) acc[b] = cross[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int turn = 0; turn < 2; ++turn) {
+    const SmBlock bl = sm_block(wave, turn);
+    if (!bl.on) continue;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f}, cross = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int st = 0; st < 2; ++st) {
-    f16x8 lf[2], rf[2];
-    sm_rows16(lf, l, 16 * (wave & 3), st, ln);
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      sm_rows16(rf, r, 32 * (wave >> 2) + 16 * b, st, ln);
-      cross[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lf[1], rf[0], cross[b], 0, 0, 0);
-      cross[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lf[0], rf[1], cross[b], 0, 0, 0);
-      acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lf[0], rf[0], acc[b], 0, 0, 0);
+    for (int st = 0; st < 2; ++st) {
+      f16x8 lf[2], rf[2];
+      sm_rows16(lf, l, bl.r0, st, ln);
+      sm_rows16(rf, r, bl.c0, st, ln);
+      cross = __builtin_amdgcn_mfma_f32_16x16x32_f16(lf[1], rf[0], cross, 0, 0, 0);
+      cross = __builtin_amdgcn_mfma_f32_16x16x32_f16(lf[0], rf[1], cross, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(lf[0], rf[0], acc, 0, 0, 0);
     }
+    v[turn] = (acc + cross) * mul;
   }
-#pragma unroll
-  for (int b = 0; b < 2; ++b) v[b] = (acc[b] + cross[b]) * mul;
 }
-// Where a lane's 4 rows of one column go: the result is symmetric, so they are 4 columns of one row, 8 B.
-__device__ __forceinline__ unsigned sm_mirror(unsigned base, int b, int wave, int lane) {
-  const int row = 32 * (wave >> 2) + 16 * b + (lane & 15), col = 16 * (wave & 3) + 4 * (lane >> 4);
-  return sm_at(base, 256, row, chunk_of(col)) + static_cast<unsigned>(2 * (col & 7));
+// Of the mirror image, a lane has four columns of one row: 8 B.
+__device__ __forceinline__ unsigned sm_mirror(unsigned base, const SmBlock& bl, int lane) {
+  const int col = bl.r0 + 4 * (lane >> 4);
+  return sm_at(base, 256, bl.c0 + (lane & 15), chunk_of(col)) + static_cast<unsigned>(2 * (col & 7));
 }
 __device__ __forceinline__ void sm_put(unsigned base, const f32x4 (&v)[2], int wave, int lane) {
   const int ln = anew(lane);
 #pragma unroll
-  for (int b = 0; b < 2; ++b) {
+  for (int turn = 0; turn < 2; ++turn) {
+    const SmBlock bl = sm_block(wave, turn);
+    if (!bl.on) continue;
     f16x4 hi, lo;
+    const int col = bl.c0 + (ln & 15), row = bl.r0 + 4 * (ln >> 4);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const Pair p = split_pair(v[b][e]);
+      const Pair p = split_pair(v[turn][e]);
       hi[e] = p.hi;
       lo[e] = p.lo;
+      const unsigned at = sm_at(base, 256, row + e, chunk_of(col)) + static_cast<unsigned>(2 * (col & 7));
+      *lds_ptr<lds_f16>(at) = p.hi;
+      *lds_ptr<lds_f16>(at ^ 64) = p.lo;
     }
-    const unsigned at = sm_mirror(base, b, wave, ln);
-    *lds_ptr<lds_f16x4>(at) = hi;
-    *lds_ptr<lds_f16x4>(at ^ 64) = lo;
+    if (bl.r0 != bl.c0) {
+      const unsigned at = sm_mirror(base, bl, ln);
+      *lds_ptr<lds_f16x4>(at) = hi;
+      *lds_ptr<lds_f16x4>(at ^ 64) = lo;
+    }
   }
 }
 
@@ -974,19 +991,26 @@ __global__ __launch_bounds__(kSmallThreads, 1) void ns_small_kernel(NsItems its,
       __syncthreads();
       if (!part) {
         const float mul = ldexpf(1.f / kScale, -2 * x_shift(tg, pl.grown[p]));
+        if (bi <= bc) {  // the block below the diagonal is the one above it, mirrored
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {  // four rows of a column, stored as the mirror image's four columns
-          f16x4 hi, lo;
+          for (int q = 0; q < 4; ++q) {  // four rows of a column: the mirror image's four columns of a row
+            f16x4 hi, lo;
+            const int row = bi + 8 * q + 4 * h, col = bc + j;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const Pair pr = split_pair(((acc[4 * q + e] + cross[4 * q + e]) + sum[64 * (4 * q + e)]) * mul);
-            hi[e] = pr.hi;
-            lo[e] = pr.lo;
+            for (int e = 0; e < 4; ++e) {
+              const Pair pr = split_pair(((acc[4 * q + e] + cross[4 * q + e]) + sum[64 * (4 * q + e)]) * mul);
+              hi[e] = pr.hi;
+              lo[e] = pr.lo;
+              const unsigned at = sm_at(MA, 256, row + e, chunk_of(col)) + static_cast<unsigned>(2 * (col & 7));
+              *lds_ptr<lds_f16>(at) = pr.hi;
+              *lds_ptr<lds_f16>(at ^ 64) = pr.lo;
+            }
+            if (bi < bc) {
+              const unsigned at = sm_at(MA, 256, col, chunk_of(row)) + static_cast<unsigned>(2 * (row & 7));
+              *lds_ptr<lds_f16x4>(at) = hi;
+              *lds_ptr<lds_f16x4>(at ^ 64) = lo;
+            }
           }
-          const int col = bi + 8 * q + 4 * h;
-          const unsigned at = sm_at(MA, 256, bc + j, chunk_of(col)) + static_cast<unsigned>(2 * (col & 7));
-          *lds_ptr<lds_f16x4>(at) = hi;
-          *lds_ptr<lds_f16x4>(at ^ 64) = lo;
         }
       }
       __syncthreads();
@@ -1001,15 +1025,17 @@ __global__ __launch_bounds__(kSmallThreads, 1) void ns_small_kernel(NsItems its,
       {
         const int ln = anew(lane);
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const unsigned at = sm_mirror(MA, b, wave, ln);
+        for (int turn = 0; turn < 2; ++turn) {
+          const SmBlock bl = sm_block(wave, turn);
+          if (!bl.on) continue;
+          const unsigned at = sm_mirror(MA, bl, ln);
           const f16x4 ah = *lds_ptr<lds_f16x4>(at), al = *lds_ptr<lds_f16x4>(at ^ 64);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float x = (static_cast<float>(ah[e]) + static_cast<float>(al[e])) * (1.f / kScale);
-            v[b][e] = fmaf(pl.c, v[b][e], pl.b * x);
-            if (16 * (wave & 3) + 4 * (ln >> 4) + e == 32 * (wave >> 2) + 16 * b + (ln & 15)) v[b][e] += pl.a;
-            v[b][e] *= sp;
+            v[turn][e] = fmaf(pl.c, v[turn][e], pl.b * x);
+            if (bl.r0 + 4 * (ln >> 4) + e == bl.c0 + (ln & 15)) v[turn][e] += pl.a;
+            v[turn][e] *= sp;
           }
         }
       }
@@ -1103,15 +1129,26 @@ float scale_for(double most) {  // the largest power of two up to kScale that ke
   return s;
 }
 
+// The longest phase for a result of 22 bits or more: A's rounding, amplified along a phase, falls on the small
+// singular directions, and near-square matrices have them. Error of five steps over that of f32 products,
+// noise matrices: phases of 3 + 2 1.5 (64 x 128), 1.7 (64 x 64); 2 + 2 + 1 0.6 and 1.4; 1 + 1 + 1 + 1 + 1
+// 0.5 and 0.6. Single steps cost no more where n < 1.5 m. A 16-bit result, and an update that is scaled
+// into the parameters, do not show the difference: 3 + 2 there (two products of m^2 n less).
+constexpr int kLongest = 3;
+int ns_exact_longest(int rows, int cols) {
+  const long long m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
+  return 2 * n < 3 * m ? 1 : 2;
+}
+
 // Phases, and scales that keep every f16 in range: the singular values of X0 are at most 1 (the Frobenius
 // norm is), the scalar map carries that bound on, and P and Q are functions of the Gram matrix.
-int ns_plan(NsPlan& pl, int steps, float a, float b, float c) {
+int ns_plan(NsPlan& pl, int steps, float a, float b, float c, int limit) {
   if (steps < 1 || steps > kMaxSteps) return fail(PROTOSEG_ERR_INVALID, "orthogonalize steps %d (1..%d)", steps, kMaxSteps);
   if (!(std::isfinite(a) && std::isfinite(b) && std::isfinite(c)))
     return fail(PROTOSEG_ERR_INVALID, "orthogonalize coefficients (%g, %g, %g)", a, b, c);
   pl.a = a, pl.b = b, pl.c = c;
   int longest = 1;  // 2^-22 a^(2 (L - 1)) <= 2^-13
-  for (double f = 1.0; longest < 3 && f * a * a <= 512.0; ++longest) f *= static_cast<double>(a) * a;
+  for (double f = 1.0; longest < limit && f * a * a <= 512.0; ++longest) f *= static_cast<double>(a) * a;
   pl.nphase = (steps + longest - 1) / longest;
   for (int p = 0, left = steps; p < pl.nphase; ++p) {
     pl.phases[p] = (left + pl.nphase - p - 1) / (pl.nphase - p);
@@ -1423,7 +1460,7 @@ extern "C" int protoseg_orthogonalize(const void* g, int dtype, int count, int r
   if (int e = ns_check(rows, cols)) return e;
   if (!(eps >= 0.f)) return fail(PROTOSEG_ERR_INVALID, "orthogonalize eps %g", eps);
   NsPlan pl;
-  if (int e = ns_plan(pl, steps, a, b, c)) return e;
+  if (int e = ns_plan(pl, steps, a, b, c, dtype == PROTOSEG_F32 ? ns_exact_longest(rows, cols) : kLongest)) return e;
   if (count == 0 || rows == 0 || cols == 0) return PROTOSEG_OK;
   const long long size = static_cast<long long>(rows) * cols;
   if (!g || !out) return fail(PROTOSEG_ERR_INVALID, "orthogonalize: matrices and result must be non-null");
@@ -1494,7 +1531,7 @@ extern "C" int protoseg_muon_step(int n_tensors, float* const* params, const flo
     return fail(PROTOSEG_ERR_INVALID, "muon: momentum %g in [0, 1), eps %g >= 0, lr %g, weight decay %g", momentum, eps, lr, weight_decay);
   if (scale_kind != 0 && scale_kind != 1) return fail(PROTOSEG_ERR_INVALID, "muon scale kind %d (0 or 1)", scale_kind);
   NsPlan pl;
-  if (int e = ns_plan(pl, steps, a, b, c)) return e;
+  if (int e = ns_plan(pl, steps, a, b, c, kLongest)) return e;
   std::vector<MuonRun> runs;
   if (int e = muon_runs(runs, n_tensors, rows, cols)) return e;
   size_t need = 0;
