@@ -1417,13 +1417,13 @@ int ns_small(const std::vector<NsItem>& items, const NsPlan& pl, float mu, int n
 // Sums of squares and X0 of all items, kMaxItems a launch.
 template <typename T, bool STEP>
 int ns_load(const NsGroups& gs, const std::vector<NsItem>& items, float mu, int nesterov, float eps, hipStream_t st) {
-  for (int pass = 0; pass < 2; ++pass)
-    for (size_t i0 = 0; i0 < items.size(); i0 += kMaxItems) {
+  for (size_t i0 = 0; i0 < items.size(); i0 += kMaxItems)
+    for (int pass = 0; pass < 2; ++pass) {  // the second pass finds what the first one read in the last-level cache
       NsItems its{};
       long long blocks = 0;
       for (int k = 0; k < kMaxItems; ++k) its.first[k] = 0x7fffffff;
       for (size_t i = i0; i < items.size() && i < i0 + kMaxItems; ++i) {
-        NsItem it = items[i];
+        const NsItem& it = items[i];
         const NsGroup& g = gs.g[it.group];
         its.first[its.n] = static_cast<int>(blocks);
         blocks += static_cast<long long>(it.count) * (pass ? static_cast<long long>(g.mp / 64) * (g.np / 64) : g.chunks);
