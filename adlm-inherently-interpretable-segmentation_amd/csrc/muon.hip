@@ -24,6 +24,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <exception>
 #include <type_traits>
 #include <utility>
 #include <vector>
@@ -1445,15 +1446,18 @@ int ns_load(const NsGroups& gs, const std::vector<NsItem>& items, float mu, int 
 
 using namespace protoseg;
 
-extern "C" size_t protoseg_orthogonalize_workspace_size(int count, int rows, int cols) {
+// No C++ exception leaves a C entry: the only ones here are allocation failures of the host lists.
+extern "C" size_t protoseg_orthogonalize_workspace_size(int count, int rows, int cols) try {
   if (count <= 0 || rows <= 0 || cols <= 0 || ns_check(rows, cols) != PROTOSEG_OK) return 0;
   NsGroups gs;
   return ns_is_small(rows, cols) ? 0 : ns_layout(gs, {NsMatrix{rows, cols, count}}, nullptr, nullptr);
+} catch (const std::exception&) {
+  return 0;
 }
 
 extern "C" int protoseg_orthogonalize(const void* g, int dtype, int count, int rows, int cols, int64_t stride, int steps, float a,
                                       float b, float c, float eps, void* out, void* workspace, size_t workspace_bytes,
-                                      protoseg_stream_t stream) {
+                                      protoseg_stream_t stream) try {
   if (dtype != PROTOSEG_F32 && dtype != PROTOSEG_BF16 && dtype != PROTOSEG_F16)
     return fail(PROTOSEG_ERR_UNSUPPORTED, "orthogonalize dtype %d (f32, bf16 or f16)", dtype);
   if (count < 0) return fail(PROTOSEG_ERR_INVALID, "orthogonalize: %d matrices", count);
@@ -1481,6 +1485,8 @@ extern "C" int protoseg_orthogonalize(const void* g, int dtype, int count, int r
   if (dtype == PROTOSEG_F32) return go(float{}, std::integral_constant<int, kOutF32>());
   if (dtype == PROTOSEG_BF16) return go(__bf16{}, std::integral_constant<int, kOutBF16>());
   return go(_Float16{}, std::integral_constant<int, kOutF16>());
+} catch (const std::exception& e) {
+  return fail(PROTOSEG_ERR_INVALID, "orthogonalize: %s", e.what());
 }
 
 namespace {
@@ -1509,7 +1515,7 @@ int muon_runs(std::vector<MuonRun>& runs, int n, const int32_t* rows, const int3
 }
 }  // namespace
 
-extern "C" size_t protoseg_muon_workspace_size(int n_tensors, const int32_t* rows, const int32_t* cols) {
+extern "C" size_t protoseg_muon_workspace_size(int n_tensors, const int32_t* rows, const int32_t* cols) try {
   std::vector<MuonRun> runs;
   if (n_tensors <= 0 || !rows || !cols || muon_runs(runs, n_tensors, rows, cols) != PROTOSEG_OK) return 0;
   size_t most = 0;
@@ -1519,12 +1525,14 @@ extern "C" size_t protoseg_muon_workspace_size(int n_tensors, const int32_t* row
     most = n > most ? n : most;
   }
   return most;
+} catch (const std::exception&) {
+  return 0;
 }
 
 extern "C" int protoseg_muon_step(int n_tensors, float* const* params, const float* const* grads, float* const* momentum_bufs,
                                   const int32_t* rows, const int32_t* cols, float momentum, int nesterov, float lr,
                                   float weight_decay, int scale_kind, int steps, float a, float b, float c, float eps,
-                                  void* workspace, size_t workspace_bytes, protoseg_stream_t stream) {
+                                  void* workspace, size_t workspace_bytes, protoseg_stream_t stream) try {
   if (n_tensors < 0 || (n_tensors > 0 && (!params || !grads || !momentum_bufs || !rows || !cols)))
     return fail(PROTOSEG_ERR_INVALID, "muon: %d tensors, pointer and size arrays must be non-null", n_tensors);
   if (!(momentum >= 0.f && momentum < 1.f) || !(eps >= 0.f) || !std::isfinite(lr) || !std::isfinite(weight_decay))
@@ -1567,4 +1575,6 @@ extern "C" int protoseg_muon_step(int n_tensors, float* const* params, const flo
   for (int i = 0; i < n_tensors; ++i)
     if (rows[i] && cols[i]) items.push_back(item(i, 0, 0));
   return ns_small<float, true>(items, pl, momentum, nesterov ? 1 : 0, eps, st);
+} catch (const std::exception& e) {
+  return fail(PROTOSEG_ERR_INVALID, "muon: %s", e.what());
 }

@@ -72,6 +72,54 @@ def test_orthogonalize(device, shape, dtype):
     check(out, g)
 
 
+def check_batch(out, g):
+    """check() of every matrix of a batch, float64 on the GPU."""
+    a, b, c = NS
+    x = g.double()
+    tall = x.shape[1] > x.shape[2]
+    x = x.transpose(1, 2).contiguous() if tall else x
+    x = x / (torch.linalg.vector_norm(x, dim=(1, 2), keepdim=True) + 1e-7)
+    norms = lambda t: torch.linalg.vector_norm(t, dim=(1, 2))  # noqa: E731
+    bound = torch.zeros(x.shape[0], dtype=torch.float64, device=x.device)
+    for _ in range(5):
+        bound = LIP * (bound + ROUNDINGS * 2.0 ** -22 * norms(x))
+        s = torch.bmm(x, x.transpose(1, 2).contiguous())
+        x = a * x + torch.bmm(b * s + c * torch.bmm(s, s), x)
+    bound += (ROUNDINGS * 2.0 ** -22 + HALF[out.dtype]) * norms(x)
+    x = x.transpose(1, 2) if tall else x
+    assert bool((norms(out.double() - x) <= bound).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [
+    (300, 30, 61),      # one workgroup a matrix
+    (1, 64, 384), (1, 385, 64),  # the largest of those, and the first beyond
+    (2, 512, 700),      # 32 x 32 tiles, the contraction over the waves
+    (1, 64, 18432), (1, 20001, 70),  # the same with a split contraction
+    (30, 130, 200),     # 64 x 64 tiles
+    (12, 200, 2100), (12, 2100, 200),  # with a split contraction
+    (100, 257, 130), (100, 130, 257),  # 128 x 128 tiles of Q X
+], ids=str)
+def test_every_kernel_path(device, shape, dtype):
+    from protoseg_amd import optim
+    gen = torch.Generator(device=device).manual_seed(21)
+    g = torch.randn(shape, generator=gen, device=device).to(dtype)
+    check_batch(optim.orthogonalize(g), g)
+
+
+def test_a_matrix_beyond_32_bit_offsets_of_its_neighbours(device):
+    """Two matrices 2^31 elements apart in memory, and one of 1.2e8 elements."""
+    from protoseg_amd import optim
+    far = torch.zeros(2 ** 31 + 70 * 90, dtype=torch.bfloat16, device=device)
+    g = far.as_strided((2, 70, 90), (2 ** 31, 90, 1))
+    g.copy_(matrix((2, 70, 90), 22).to(torch.bfloat16))
+    check_batch(optim.orthogonalize(g), g)
+    del far, g
+    gen = torch.Generator(device=device).manual_seed(23)
+    g = torch.randn((1, 40, 3_000_001), generator=gen, device=device)
+    check_batch(optim.orthogonalize(g), g)
+
+
 @pytest.mark.parametrize("kind", ["spiked", "rank1", "graded"])
 @pytest.mark.parametrize("shape", [(96, 200), (200, 96), (128, 128)], ids=str)
 def test_conditioning(device, shape, kind):

@@ -177,6 +177,39 @@ def test_without_weight_or_bias(device, which):
         close(gw, ref, "gw")
 
 
+def test_map_beyond_32_bit_offsets(device):
+    """2.2e9 elements (bf16): statistics from f64 sums of slabs, y and the gradients at the far end."""
+    from protoseg_amd import norm
+    C, H, W, groups = 64, 5860, 5860, 8
+    gen = torch.Generator(device=device).manual_seed(3)
+    x = torch.empty((1, H, W, C), dtype=torch.bfloat16, device=device)
+    for part in x[0].chunk(20):
+        part.copy_(torch.randn(part.shape, generator=gen, device=device) + 0.5)
+    x = x.permute(0, 3, 1, 2)
+    assert x.numel() > 2 ** 31
+    y, stats = norm.group_norm_forward(x, None, None, groups, 1e-5, 2)
+    total = sum(p.double().reshape(-1, groups, C // groups).sum((0, 2)) for p in x[0].permute(1, 2, 0).chunk(20))
+    square = sum(p.double().square().reshape(-1, groups, C // groups).sum((0, 2)) for p in x[0].permute(1, 2, 0).chunk(20))
+    M = H * W * (C // groups)
+    mean, var = total / M, square / M - (total / M) ** 2
+    rstd = 1 / (var + 1e-5).sqrt()
+    assert torch.allclose(stats[0, :, 0], mean, rtol=1e-12, atol=0) and torch.allclose(stats[0, :, 1], rstd, rtol=1e-12, atol=0)
+    m, r = (v.repeat_interleave(C // groups) for v in (mean, rstd))
+    last = (x[0, :, -3:].double().permute(1, 2, 0) - m) * r
+    ref = torch.sigmoid(last)
+    err = (y[0, :, -3:].double().permute(1, 2, 0) - ref).abs()
+    # half a step of bf16: finfo.eps = 2^-7 between 1 and 2, so 2^-8 of the value
+    assert bool((err <= (2.0 ** -8 + 4 * U * (last.abs() + 4)) * ref).all())
+    gx, gw, gb = norm.group_norm_backward(x, y, None, None, stats, groups, 2)
+    # gb of y itself: sum of y * y (1 - y) with the f64 sigmoid of z; every term is positive
+    want = torch.zeros(C, dtype=torch.float64, device=device)
+    for px, py in zip(x[0].permute(1, 2, 0).chunk(40), y[0].permute(1, 2, 0).chunk(40)):
+        s = torch.sigmoid((px.double() - m) * r)
+        want += (py.double() * s * (1 - s)).sum((0, 1))
+    assert bool(((gb.double() - want).abs() <= 3 * CHAIN * U * want).all())
+    assert bool(torch.isfinite(gx[0, :, -1]).all()) and bool((gx[0, :, -1] != 0).any())
+
+
 def test_mean_far_larger_than_the_spread(device):
     """|mean| about 3000 spreads in f32: the statistics and x - mean keep full precision."""
     x, w, b, gy = make(device, 2, 32, 21, 19, torch.float32, 23, mean=3000.0)

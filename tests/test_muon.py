@@ -10,14 +10,14 @@ NULL, SOME = ctypes.c_void_p(None), ctypes.c_void_p(4096)
 NS = optim.NS_COEFFICIENTS
 
 
-def orth(g=SOME, dtype=0, count=1, rows=4, cols=6, stride=24, steps=5, abc=NS, eps=1e-7, out=SOME, ws=NULL, nbytes=0):
+def orth(g=SOME, dtype=0, count=1, rows=100, cols=200, stride=20000, steps=5, abc=NS, eps=1e-7, out=SOME, ws=NULL, nbytes=0):
     return _lib.load().protoseg_orthogonalize(g, dtype, count, rows, cols, stride, steps, *abc, eps, out, ws, nbytes, NULL)
 
 
 @pytest.mark.parametrize("bad, status, text", [
     (dict(dtype=2), _lib.ERR_UNSUPPORTED, b"dtype"),
     (dict(count=-1), _lib.ERR_INVALID, b"-1 matrices"),
-    (dict(rows=-2), _lib.ERR_INVALID, b"-2 x 6"),
+    (dict(rows=-2), _lib.ERR_INVALID, b"-2 x 200"),
     (dict(rows=40000, cols=40000), _lib.ERR_UNSUPPORTED, b"at most"),
     (dict(rows=17000, cols=17000), _lib.ERR_UNSUPPORTED, b"at most"),
     (dict(steps=0), _lib.ERR_INVALID, b"steps"),
@@ -28,7 +28,7 @@ def orth(g=SOME, dtype=0, count=1, rows=4, cols=6, stride=24, steps=5, abc=NS, e
     (dict(eps=float("nan")), _lib.ERR_INVALID, b"eps"),
     (dict(g=NULL), _lib.ERR_INVALID, b"non-null"),
     (dict(out=NULL), _lib.ERR_INVALID, b"non-null"),
-    (dict(count=2, stride=23), _lib.ERR_INVALID, b"overlap"),
+    (dict(count=2, stride=19999), _lib.ERR_INVALID, b"overlap"),
     (dict(), _lib.ERR_INVALID, b"workspace"),
 ])
 def test_orthogonalize_refusals(bad, status, text):
@@ -47,23 +47,27 @@ def test_empty_calls_need_nothing():
 def test_muon_refusals():
     lib = _lib.load()
 
-    def step(n=1, mu=0.9, eps=1e-7, kind=0, steps=5, rows=4, null=False):
+    def step(n=1, mu=0.9, eps=1e-7, kind=0, steps=5, rows=100, null=False):
         ptrs = (ctypes.c_void_p * 1)(None if null else 4096)
-        r, c = (ctypes.c_int32 * 1)(rows), (ctypes.c_int32 * 1)(6)
+        r, c = (ctypes.c_int32 * 1)(rows), (ctypes.c_int32 * 1)(200)
         return lib.protoseg_muon_step(n, ptrs, ptrs, ptrs, r, c, mu, 1, 0.1, 0.0, kind, steps, *NS, eps, NULL, 0, NULL)
 
     for bad, text in ((dict(n=-1), b"-1 tensors"), (dict(mu=1.0), b"momentum"), (dict(eps=-1.0), b"eps"), (dict(kind=2), b"scale"),
-                      (dict(steps=0), b"steps"), (dict(rows=-1), b"-1 x 6"), (dict(null=True), b"null pointer"), (dict(), b"workspace")):
+                      (dict(steps=0), b"steps"), (dict(rows=-1), b"-1 x 200"), (dict(null=True), b"null pointer"), (dict(), b"workspace")):
         assert step(**bad) == _lib.ERR_INVALID and text in lib.protoseg_last_error(), bad
 
 
 def test_workspace_covers_every_run_of_shapes():
     lib = _lib.load()
     n = 60
-    rows, cols = (ctypes.c_int32 * n)(*range(8, 8 + n)), (ctypes.c_int32 * n)(*range(70, 70 + n))
+    rows, cols = (ctypes.c_int32 * n)(*range(80, 80 + n)), (ctypes.c_int32 * n)(*range(90, 90 + n))
     whole = lib.protoseg_muon_workspace_size(n, rows, cols)
     first = lib.protoseg_muon_workspace_size(24, rows, cols)
     assert 0 < first <= whole and whole % 256 == 0
+    # matrices that one workgroup takes whole need none
+    assert lib.protoseg_orthogonalize_workspace_size(7, 361, 64) == 0 < lib.protoseg_orthogonalize_workspace_size(7, 385, 64)
+    small_r, small_c = (ctypes.c_int32 * 2)(361, 19), (ctypes.c_int32 * 2)(64, 361)
+    assert lib.protoseg_muon_workspace_size(2, small_r, small_c) == 0
 
 
 def test_python_refusals():
