@@ -14,6 +14,7 @@ may be alive while it is captured.
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -26,28 +27,24 @@ from .ops import _x_dtype
 ACTIVATIONS = {"identity": 0, "relu": 1, "sigmoid": 2, "silu": 3}
 
 
-def _rows(x: Tensor) -> Tensor:
-    """x as the kernels read it: channel stride 1, one stride from pixel to pixel. A channels-last
-    map, and a slice of one along batch or channels, passes as it is; anything else is copied."""
+def _rows(x: Tensor) -> Tuple[Tensor, int, int]:
+    """x as the kernels read it, channel stride 1 and one stride from pixel to pixel, with its sample
+    and pixel strides. A channels-last map, and a slice of one along batch or channels, passes as it
+    is; anything else is copied. A stride that is never stepped over is given its dense value."""
     B, C, H, W = x.shape
     sb, sc, sh, sw = x.stride()
-    rows = (sc == 1 or C == 1) and (W == 1 or sw >= C) and (H == 1 or (sh == sw * W if W > 1 else sh >= C))
-    if rows and (B == 1 or sb >= _pixel_stride(x) * (H * W - 1) + C):
-        return x
-    return x.contiguous(memory_format=torch.channels_last)
+    sp = sw if W > 1 else sh if H > 1 else C
+    if (sc == 1 or C == 1) and sp >= C and (H == 1 or W == 1 or sh == sw * W):
+        if B == 1:
+            return x, H * W * sp, sp
+        if sb >= sp * (H * W - 1) + C:
+            return x, sb, sp
+    return x.contiguous(memory_format=torch.channels_last), H * W * C, C
 
 
-def _pixel_stride(x: Tensor) -> int:
-    _, C, H, W = x.shape
-    return x.stride(3) if W > 1 else x.stride(2) if H > 1 else C
-
-
-def _strides(x: Tensor) -> Tuple[int, int]:
-    """(sample, pixel) strides in elements of a map that _rows returned. A contiguous 1-channel or
-    1-pixel map may carry any stride there; what is never stepped over is given its dense value."""
-    B, C, H, W = x.shape
-    sp = _pixel_stride(x)
-    return (x.stride(0) if B > 1 else H * W * sp), sp
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(code: int, B: int, HW: int, C: int, groups: int, backward: int) -> int:
+    return _lib.load().protoseg_group_norm_workspace_size(code, B, HW, C, groups, backward)
 
 
 def _empty_like_map(x: Tensor) -> Tensor:
@@ -62,9 +59,10 @@ def _check(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tens
     C = x.shape[1]
     if groups < 1 or C < 1 or C % groups:
         raise _lib.ProtosegError(f"{C} channels do not divide into {groups} groups")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (C,)):
-            raise _lib.ProtosegError(f"group norm {name}: float32 [{C}] expected, got {t.dtype} {tuple(t.shape)}")
+    if weight is not None and (weight.dtype != torch.float32 or weight.shape != (C,)):
+        raise _lib.ProtosegError(f"group norm weight: float32 [{C}] expected, got {weight.dtype} {tuple(weight.shape)}")
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (C,)):
+        raise _lib.ProtosegError(f"group norm bias: float32 [{C}] expected, got {bias.dtype} {tuple(bias.shape)}")
     if act not in ACTIVATIONS.values():
         raise _lib.ProtosegError(f"activation code {act} unknown")
     return code
@@ -74,19 +72,19 @@ def _forward(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], groups
     """y, stats and what a backward needs again: (x, weight, bias as read; the call's sizes)."""
     code = _check(x, groups, weight, bias, act)
     dev = _lib.require_device(x, weight, bias)
-    x = _rows(x)
+    x, sb, sp = _rows(x)
     weight = weight.contiguous() if weight is not None else None
     bias = bias.contiguous() if bias is not None else None
     B, C, H, W = x.shape
     y = _empty_like_map(x)
     stats = torch.empty((B, groups, 2), device=dev, dtype=torch.float64)
-    sizes = (code, B, H * W, C, *_strides(x))
+    sizes = (code, B, H * W, C, sb, sp)
     if x.numel() == 0:
         stats.zero_()
     else:
         lib = _lib.load()
         with _lib.on_device(dev):
-            nbytes = lib.protoseg_group_norm_workspace_size(code, B, H * W, C, groups, 0)
+            nbytes = _workspace_bytes(code, B, H * W, C, groups, 0)
             ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
             _lib.check("protoseg_group_norm_fwd", lib.protoseg_group_norm_fwd(
                 x.data_ptr(), *sizes, groups, _lib.addr(weight), _lib.addr(bias), eps, act, y.data_ptr(), stats.data_ptr(),
@@ -98,7 +96,7 @@ def _backward(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], stats
               act: int, need_x: bool, need_weight: bool, need_bias: bool):
     """The backward on tensors that _forward returned; only g_y is new to it."""
     dev = x.device
-    g_y = _rows(g_y if g_y.dtype == x.dtype else g_y.to(x.dtype))
+    g_y, gsb, gsp = _rows(g_y if g_y.dtype == x.dtype else g_y.to(x.dtype))
     C = sizes[3]
     g_x = _empty_like_map(x) if need_x else None
     if x.numel() == 0:
@@ -108,10 +106,10 @@ def _backward(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], stats
     g_b = torch.empty(C, device=dev, dtype=torch.float32) if need_bias else None
     lib = _lib.load()
     with _lib.on_device(dev):
-        nbytes = lib.protoseg_group_norm_workspace_size(*sizes[:4], groups, 1)
+        nbytes = _workspace_bytes(*sizes[:4], groups, 1)
         ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
         _lib.check("protoseg_group_norm_bwd", lib.protoseg_group_norm_bwd(
-            x.data_ptr(), g_y.data_ptr(), *sizes, *_strides(g_y), groups, _lib.addr(weight), _lib.addr(bias), act,
+            x.data_ptr(), g_y.data_ptr(), *sizes, gsb, gsp, groups, _lib.addr(weight), _lib.addr(bias), act,
             stats.data_ptr(), _lib.addr(g_x), _lib.addr(g_w), _lib.addr(g_b), ws.data_ptr(), nbytes, _lib.stream_of(dev)))
     return g_x, g_w, g_b
 
@@ -130,10 +128,10 @@ def group_norm_backward(x: Tensor, g_y: Tensor, weight: Optional[Tensor], bias: 
     _lib.require_device(x, g_y, weight, bias, stats)
     if g_y.shape != x.shape or stats.dtype != torch.float64 or tuple(stats.shape) != (x.shape[0], groups, 2):
         raise _lib.ProtosegError("group norm backward: g_y and stats must be of the forward's shapes")
-    x = _rows(x)
+    x, sb, sp = _rows(x)
     B, C, H, W = x.shape
     return _backward(x, weight.contiguous() if weight is not None else None, bias.contiguous() if bias is not None else None,
-                     stats.contiguous(), (code, B, H * W, C, *_strides(x)), g_y, groups, act, need_x, need_weight, need_bias)
+                     stats.contiguous(), (code, B, H * W, C, sb, sp), g_y, groups, act, need_x, need_weight, need_bias)
 
 
 class _GroupNorm(torch.autograd.Function):
@@ -147,8 +145,9 @@ class _GroupNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g_y):
+        if torch.is_grad_enabled():  # create_graph
+            raise _lib.ProtosegError("group norm has no second derivative")
         return (*_backward(*ctx.saved_tensors, ctx.sizes, g_y, ctx.groups, ctx.act, *ctx.needs_input_grad[:3]), None, None, None)
 
 
@@ -170,7 +169,8 @@ def group_norm(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias: Op
     if bias is not None and bias.dtype != torch.float32 and bias.is_floating_point():
         bias = bias.float()
     args = (x, weight, bias, int(groups), float(eps), ACTIVATIONS[activation])
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:3]):
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
         return _GroupNorm.apply(*args)
     return group_norm_forward(*args)[0]
 

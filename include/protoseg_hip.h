@@ -609,8 +609,8 @@ int protoseg_group_norm_bwd(const void* x, const void* g_y, int x_dtype, int B, 
  * Arithmetic: f32-class (f16 pairs, f32 accumulation) for every dtype; a 16-bit result is rounded once. A zero
  * matrix gives zeros; a value that is not finite makes its own matrix NaN. Coefficients under which a
  * singular value in [0, 1] could grow to 4 are refused (PROTOSEG_ERR_UNSUPPORTED). No atomics: the same bits
- * on every run. workspace: protoseg_orthogonalize_workspace_size(...) bytes, 256-B aligned, of one call
- * at a time.
+ * on every run. workspace: protoseg_orthogonalize_workspace_size(...) bytes (0 for matrices that one
+ * workgroup takes whole), 256-B aligned, of one call at a time.
  */
 size_t protoseg_orthogonalize_workspace_size(int count, int rows, int cols);
 int protoseg_orthogonalize(const void* g, int dtype, int count, int rows, int cols, int64_t stride, int steps, float a,

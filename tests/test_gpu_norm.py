@@ -343,6 +343,9 @@ def test_module_and_autocast_weights(device):
 
 def test_refusals_on_the_device(device):
     from protoseg_amd import _lib, norm
+    leaf = torch.zeros(2, 12, 4, 4, device=device, requires_grad=True)
+    with pytest.raises(_lib.ProtosegError, match="second derivative"):
+        torch.autograd.grad(norm.group_norm(leaf, 4).sum(), leaf, create_graph=True)
     x = torch.zeros(2, 12, 4, 4, device=device)
     with pytest.raises(_lib.ProtosegError, match="groups"):
         norm.group_norm(x, 5)

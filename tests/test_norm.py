@@ -66,14 +66,16 @@ def test_cpu_tensors_are_refused():
 
 def test_what_is_read_in_place():
     cl = torch.zeros(2, 24, 6, 5).contiguous(memory_format=torch.channels_last)
-    for view in (cl, cl[:, 8:16], cl[1:], cl[::2], cl[:, :, :, :1][:, :, :1]):
-        assert norm._rows(view).data_ptr() == view.data_ptr()
-    assert norm._strides(cl[:, 8:16]) == (24 * 30, 24)
+    for view in (cl, cl[:, 8:16], cl[1:], cl[::2], cl[:, :, :, :1][:, :, :1], cl[:, :, :, :1]):
+        assert norm._rows(view)[0].data_ptr() == view.data_ptr()
+    assert norm._rows(cl[:, 8:16])[1:] == (24 * 30, 24)
+    assert norm._rows(cl[:, :, :, :1])[1:] == (24 * 30, 24 * 5)  # one column: the pixel stride is the rows'
     for view in (cl[..., ::2], cl[:, :, ::2], torch.zeros(2, 24, 6, 5), cl[:1].expand(3, -1, -1, -1), cl[:, :1].expand(-1, 8, -1, -1)):
-        rows = norm._rows(view)
+        rows, sb, sp = norm._rows(view)
         assert rows.data_ptr() != view.data_ptr() and rows.is_contiguous(memory_format=torch.channels_last)
+        assert (sb, sp) == (view.shape[2] * view.shape[3] * view.shape[1], view.shape[1])
     one = torch.zeros(1, 1, 4, 3)  # a single channel is both layouts at once
-    assert norm._strides(norm._rows(one)) == (12, 1)
+    assert norm._rows(one)[1:] == (12, 1)
 
 
 def test_module_refusals():
