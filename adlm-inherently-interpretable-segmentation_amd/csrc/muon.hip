@@ -64,8 +64,8 @@ struct NsTarget {
 
 // One shape. Buffers (byte offsets from the workspace): X0, X1 [count][mp][np] pairs at x; A, P, T, Q0, Q1
 // [count][mp][mp] pairs at sq; Gram partials [count][split][mp][mp] f32 at part. Pairs are row-major, 32 hi
-// values and their 32 lo values in turn: a 32-k stage of a row is one 128-B line (with hi and lo in planes
-// of their own it was two half lines, and L2 served twice the requests).
+// values and their 32 lo values in turn: a 32-k stage of a row is one 128-B line. (With hi and lo in planes
+// of their own it was two half lines and twice the requests to L2, at the same time.)
 struct NsGroup {
   int m, n, mp, np, count, tall;
   int split;         // workgroups along the Gram contraction
@@ -161,25 +161,28 @@ __device__ __forceinline__ float src_at(const void* p, long long i) {
   return static_cast<float>(static_cast<const T*>(p)[i]);
 }
 
-// The group (item) of a workgroup. first[] is an array of its own, so that the search reads two lines of the
-// arguments and not one per group (each a trip to memory: 30 us of the backbone's step).
+// The group (item) of a workgroup: a binary search, since each probe is a scalar load that the next one
+// waits for (22 matrices of 256 x 1024: 185 us for 190 in order). first[] is an array of its own, two lines of
+// the arguments and not one per group.
 template <int N>
 __device__ __forceinline__ int place_of(const int (&first)[N], int blk) {
   int k = 0;
-  while (k + 1 < N && blk >= first[k + 1]) ++k;
+#pragma unroll
+  for (int step = 16; step; step >>= 1)
+    if (k + step < N && blk >= first[k + step < N ? k + step : 0]) k += step;
   return k;
 }
 
 // A launch gives group g n = per matrix x count workgroups, rounded up to a multiple of 8, and XCD x (which runs
 // the workgroups i % 8 == x) the x-th eighth of them in order: neighbouring tiles of a matrix share operands,
-// and an XCD finds them in its own 4 MiB L2. Spread over the XCDs, every tile's operands came from beyond
-// the L2s (8 TB/s over the chip, the bound of every product). -1: past the end.
+// and an XCD finds them in its own 4 MiB L2 (22 matrices of 256 x 1024: 193 us for 220). -1: past the end.
 __device__ __forceinline__ int xcd_local(int b, int n) {
   const int chunk = (n + 7) >> 3, i = (b & 7) * chunk + (b >> 3);
   return i < n && (b >> 3) < chunk ? i : -1;
 }
 
-// Sum of squares of one chunk of a matrix, in f64 (squares of every f32 stay in range). STEP: the momentum
+// Sum of squares of one chunk of a matrix, in f64 (squares of every f32 stay in range). Bound by memory: 122 us for
+// 47e6 elements' gradients and momentum, 4.6 TB/s. STEP: the momentum
 // B <- mu B + g is written here, and the squares are those of the update U = g + mu B (nesterov) or B.
 template <typename T, bool STEP>
 __global__ __launch_bounds__(kNormThreads) void ns_norm_kernel(NsGroups gs, NsItems its, float mu, int nesterov) {
@@ -271,7 +274,7 @@ __device__ __forceinline__ NsScale scale_of(double squares, float eps) {
 }
 
 // X0 of one 64 x 64 tile: the (update's) values over their norm, transposed where the matrix is tall, as
-// f16 pairs, zeros in the padding.
+// f16 pairs, zeros in the padding. 104 us for 47e6 elements: 5.4 TB/s, the reads from the last-level cache.
 template <typename T, bool STEP>
 __global__ __launch_bounds__(256) void ns_load_kernel(NsGroups gs, NsItems its, float mu, int nesterov, float eps) {
   __shared__ float tile[64][65];
@@ -377,8 +380,13 @@ __device__ __forceinline__ void stage_wait(int later) {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PER * MOST) : "memory");
 }
 
-// T x T output tile, 4 waves of (T / 2) x (T / 2). Three LDS stages filled by LDS-DMA two stages ahead of
-// the products (one barrier a stage); 3 MFMAs per 32 x 32 x 16 block.
+// T x T output tile, 4 waves of (T / 2) x (T / 2), 3 MFMAs per 32 x 32 x 16 block. LDS-DMA fills a ring of
+// stages of 32 k, ring_of - 1 ahead of the products, with one barrier a stage. In the step over a ResNet-101's
+// convolutions (109 matrices, 47e6 elements) the Gram product takes 113 us, Q X 145 us, Q X with the parameters'
+// update 182 us, a product of squares 31 us: 505, 662, 528 and 403 TFLOP/s of f16, where a large library product
+// reaches 1100. LDS bounds a 64 x 64 tile: a stage is 192 cycles of MFMA on each SIMD, and 32 KiB read and 16 KiB
+// written at 128 B a cycle are 384. At 128 x 128 they are even (768 and 768), but the symmetric products would
+// compute a fifth more and leave half the chip's places empty at the end (measured slower).
 template <int T, int MODE, int OUT>
 __global__ __launch_bounds__(256, 160 * 1024 / (ring_of(T) * stage_bytes(T))) void ns_product_kernel(NsGroups gs, NsJobs js) {
   constexpr int MI = T / 64, kPieces = T / 32;  // 1-KiB DMA pieces per operand and wave
@@ -598,7 +606,8 @@ __global__ __launch_bounds__(256, 160 * 1024 / (ring_of(T) * stage_bytes(T))) vo
 
 // The symmetric products of few matrices: a 32 x 32 tile a workgroup, whose 4 waves take every fourth 32-k stage
 // (a ring of 4 stages of its own each, no barrier in the loop) and then a quarter of the tile's rows each. A
-// launch of few tiles is a chain of load latencies along k: a quarter of it, and four times the workgroups.
+// launch of few tiles is a chain of load latencies along k: a quarter of it, and four times the workgroups. A
+// launch takes 6.8 us at m = 512 (64 x 64 tiles: 10) and 5.0 at m = 128, of which 2.4 are the launch alone.
 constexpr int kThinRing = 4, kThinStage = 2 * 32 * 128;
 template <int MOST>
 __device__ __forceinline__ void thin_wait(int later) {  // at most min(later, MOST) stages of 8 loads in flight
@@ -718,7 +727,8 @@ __global__ __launch_bounds__(256, 1) void ns_thin_kernel(NsGroups gs, NsJobs js)
   }
 }
 
-// The partials of a split Gram product joined in a fixed order: a workgroup takes one 32 x 32 block on or
+// The partials of a split Gram product joined in a fixed order (8.2 us in the 109 matrices' step, bound by reading
+// them): a workgroup takes one 32 x 32 block on or
 // above the diagonal, each wave every fourth split, and stores it with its mirror image.
 __global__ __launch_bounds__(256) void ns_join_kernel(NsGroups gs, float inv, int grown) {
   __shared__ float red[3][16][64];
@@ -764,8 +774,11 @@ __global__ __launch_bounds__(256) void ns_join_kernel(NsGroups gs, float inv, in
 
 // Matrices of up to 64 rows and 384 columns (padded): norm, X and all products of one matrix in one
 // workgroup, X and four 64 x 64 matrices in LDS (64 * 384 * 4 + 4 * 16 KiB = 160 KiB). Such a matrix is a
-// chain of some 20 products of well under 1 us each, and a launch each costs 4 to 5 us.
-constexpr int kSmallM = 64, kSmallN = 384, kSmallThreads = 512;
+// chain of some 20 products of about 1 us each, and a launch each costs 4 to 5 us: 361 x 64 f32 takes 35 us
+// for 92. What bounds it is the chain of LDS reads, MFMAs, LDS writes and barriers (a step 3.0 us, a Gram
+// matrix and Q X 3.3, load and store 9), so the blocks of a product lie on as many waves: 12 for 10 blocks
+// (8 waves, two of them with two blocks: 40 us).
+constexpr int kSmallM = 64, kSmallN = 384, kSmallThreads = 768;
 constexpr int kSmallSquare = 64 * 256;  // bytes of a 64 x 64 matrix of pairs
 
 struct NsPlan {
@@ -831,63 +844,53 @@ __device__ __forceinline__ int anew(int v) {
 }
 
 // The product L R^T of two symmetric 64 x 64 matrices that commute, so that it is symmetric too: the 10 blocks of
-// 16 x 16 on and above the diagonal, block w to wave w and blocks 8 and 9 to the first two again. A lane has
-// column lane & 15 and rows 4 (lane >> 4) .. + 3 of a block. Blocks above the diagonal are stored with their
-// mirror images: a result that is symmetric but for its roundings drifts, to twice the error over five steps.
+// 16 x 16 on and above the diagonal, block w to wave w. A lane has column lane & 15 and rows 4 (lane >> 4) .. + 3
+// of its block. Blocks above the diagonal are stored with their mirror images: a result that is symmetric but for
+// its roundings drifts, to twice the error over five steps.
 struct SmBlock {
   int r0, c0;
   bool on;
 };
-__device__ __forceinline__ SmBlock sm_block(int wave, int turn) {
-  const int t = wave + 8 * turn, bi = t < 4 ? 0 : t < 7 ? 1 : t < 9 ? 2 : 3, bc = t < 4 ? t : t < 7 ? t - 3 : t < 9 ? t - 5 : 3;
+__device__ __forceinline__ SmBlock sm_block(int t) {
+  const int bi = t < 4 ? 0 : t < 7 ? 1 : t < 9 ? 2 : 3, bc = t < 4 ? t : t < 7 ? t - 3 : t < 9 ? t - 5 : 3;
   return SmBlock{16 * bi, 16 * bc, t < 10};
 }
-__device__ __forceinline__ void sm_square(unsigned l, unsigned r, float mul, f32x4 (&v)[2], int wave, int lane) {
+__device__ __forceinline__ f32x4 sm_square(unsigned l, unsigned r, float mul, const SmBlock& bl, int lane) {
   const int ln = anew(lane);
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f}, cross = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int turn = 0; turn < 2; ++turn) {
-    const SmBlock bl = sm_block(wave, turn);
-    if (!bl.on) continue;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f}, cross = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int st = 0; st < 2; ++st) {
-      f16x8 lf[2], rf[2];
-      sm_rows16(lf, l, bl.r0, st, ln);
-      sm_rows16(rf, r, bl.c0, st, ln);
-      cross = __builtin_amdgcn_mfma_f32_16x16x32_f16(lf[1], rf[0], cross, 0, 0, 0);
-      cross = __builtin_amdgcn_mfma_f32_16x16x32_f16(lf[0], rf[1], cross, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(lf[0], rf[0], acc, 0, 0, 0);
-    }
-    v[turn] = (acc + cross) * mul;
+  for (int st = 0; st < 2; ++st) {
+    f16x8 lf[2], rf[2];
+    sm_rows16(lf, l, bl.r0, st, ln);
+    sm_rows16(rf, r, bl.c0, st, ln);
+    cross = __builtin_amdgcn_mfma_f32_16x16x32_f16(lf[1], rf[0], cross, 0, 0, 0);
+    cross = __builtin_amdgcn_mfma_f32_16x16x32_f16(lf[0], rf[1], cross, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(lf[0], rf[0], acc, 0, 0, 0);
   }
+  return (acc + cross) * mul;
 }
 // Of the mirror image, a lane has four columns of one row: 8 B.
 __device__ __forceinline__ unsigned sm_mirror(unsigned base, const SmBlock& bl, int lane) {
   const int col = bl.r0 + 4 * (lane >> 4);
   return sm_at(base, 256, bl.c0 + (lane & 15), chunk_of(col)) + static_cast<unsigned>(2 * (col & 7));
 }
-__device__ __forceinline__ void sm_put(unsigned base, const f32x4 (&v)[2], int wave, int lane) {
+__device__ __forceinline__ void sm_put(unsigned base, const f32x4& v, const SmBlock& bl, int lane) {
   const int ln = anew(lane);
+  f16x4 hi, lo;
+  const int col = bl.c0 + (ln & 15), row = bl.r0 + 4 * (ln >> 4);
 #pragma unroll
-  for (int turn = 0; turn < 2; ++turn) {
-    const SmBlock bl = sm_block(wave, turn);
-    if (!bl.on) continue;
-    f16x4 hi, lo;
-    const int col = bl.c0 + (ln & 15), row = bl.r0 + 4 * (ln >> 4);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const Pair p = split_pair(v[turn][e]);
-      hi[e] = p.hi;
-      lo[e] = p.lo;
-      const unsigned at = sm_at(base, 256, row + e, chunk_of(col)) + static_cast<unsigned>(2 * (col & 7));
-      *lds_ptr<lds_f16>(at) = p.hi;
-      *lds_ptr<lds_f16>(at ^ 64) = p.lo;
-    }
-    if (bl.r0 != bl.c0) {
-      const unsigned at = sm_mirror(base, bl, ln);
-      *lds_ptr<lds_f16x4>(at) = hi;
-      *lds_ptr<lds_f16x4>(at ^ 64) = lo;
-    }
+  for (int e = 0; e < 4; ++e) {
+    const Pair p = split_pair(v[e]);
+    hi[e] = p.hi;
+    lo[e] = p.lo;
+    const unsigned at = sm_at(base, 256, row + e, chunk_of(col)) + static_cast<unsigned>(2 * (col & 7));
+    *lds_ptr<lds_f16>(at) = p.hi;
+    *lds_ptr<lds_f16>(at ^ 64) = p.lo;
+  }
+  if (bl.r0 != bl.c0) {
+    const unsigned at = sm_mirror(base, bl, ln);
+    *lds_ptr<lds_f16x4>(at) = hi;
+    *lds_ptr<lds_f16x4>(at ^ 64) = lo;
   }
 }
 
@@ -900,7 +903,7 @@ __global__ __launch_bounds__(kSmallThreads, 1) void ns_small_kernel(NsItems its,
   const int mat = static_cast<int>(blockIdx.x) - its.first[k];
   const int rows = it.rows, cols = it.cols, tall = rows > cols;
   const int m = tall ? cols : rows, n = tall ? rows : cols, np = (n + 63) & ~63;
-  const int lane = threadIdx.x & 63, wave = bf16l::wave_id(), j = lane & 31, h = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = bf16l::wave_id();
   const unsigned MA = S0, MP = S0 + kSmallSquare, MQ = S0 + 2 * kSmallSquare, MT = S0 + 3 * kSmallSquare, X = S0 + 4 * kSmallSquare;
   const int xp = np * 4;  // pitch of X
   const T* src = static_cast<const T*>(it.src) + mat * it.sb;
@@ -910,33 +913,65 @@ __global__ __launch_bounds__(kSmallThreads, 1) void ns_small_kernel(NsItems its,
   // X's rows, which are one 16-B chunk of hi and one of lo: row i, columns 8 kc .. + 7.
   constexpr int kRuns = kSmallM * kSmallN / 8 / kSmallThreads;
   const int nc = (n + 7) >> 3, runs = m * nc;
-  float v0[kRuns][8];
+  struct SmRun {
+    int i, kc, at, step, left;  // row, chunk; its first value's place, the next one's distance, values there are
+    bool on;
+  };
   int place[kRuns];  // i + 64 kc
+#pragma unroll
+  for (int q = 0; q < kRuns; ++q) {
+    const int id = min(static_cast<int>(threadIdx.x) + q * kSmallThreads, runs - 1);
+    place[q] = tall ? id % m + 64 * (id / m) : id / nc + 64 * (id % nc);
+  }
+  auto run_of = [&](int q) __attribute__((always_inline)) {
+    const int i = place[q] & 63, kc = place[q] >> 6;
+    return SmRun{i, kc, tall ? 8 * kc * cols + i : i * cols + 8 * kc, tall ? cols : 1, n - 8 * kc,
+                 static_cast<int>(threadIdx.x) + q * kSmallThreads < runs};
+  };
+  // Whole runs of a wide matrix's aligned rows in 16-B loads (64 x 384 f32: 32.7 us
+  // for 42.1 us one by one).
+  typedef T vec8 __attribute__((ext_vector_type(8)));
+  typedef float f32x8 __attribute__((ext_vector_type(8)));
+  const bool vec = !tall && cols % 8 == 0 && ((reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(buf)) & 31) == 0;
+  float v0[kRuns][8], o[kRuns][8];
+#pragma unroll
+  for (int q = 0; q < kRuns; ++q) {  // all loads in flight at once
+    if (q * kSmallThreads < runs) {
+      const SmRun r = run_of(q);
+      if (vec) {
+        const vec8 x = *reinterpret_cast<const vec8*>(src + r.at);
+        f32x8 y;
+        if constexpr (STEP) y = *reinterpret_cast<const f32x8*>(buf + r.at);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v0[q][e] = static_cast<float>(x[e]);
+          if constexpr (STEP) o[q][e] = y[e];
+        }
+        continue;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int a = r.at + min(e, r.left - 1) * r.step;
+        v0[q][e] = src_at<T>(src, a);
+        if constexpr (STEP) o[q][e] = buf[a];
+      }
+    }
+  }
   double s = 0.0;
 #pragma unroll
   for (int q = 0; q < kRuns; ++q) {
     if (q * kSmallThreads < runs) {
-      const int id = static_cast<int>(threadIdx.x) + q * kSmallThreads, idc = min(id, runs - 1);
-      const int kc = tall ? idc / m : idc % nc, i = tall ? idc % m : idc / nc;
-      place[q] = i + 64 * kc;
-      const int at = tall ? 8 * kc * cols + i : i * cols + 8 * kc, step = tall ? cols : 1, left = n - 8 * kc;
-      float x[8], o[8];
+      pin_batch(v0[q]);
+      if constexpr (STEP) pin_batch(o[q]);
+      const SmRun r = run_of(q);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int a = at + min(e, left - 1) * step;
-        x[e] = src_at<T>(src, a);
-        if constexpr (STEP) o[e] = buf[a];
-      }
-      pin_batch(x);
-      if constexpr (STEP) pin_batch(o);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const bool in = id < runs && e < left;
-        float w = x[e];
+        const bool in = r.on && e < r.left;
+        float w = v0[q][e];
         if constexpr (STEP) {
-          const float nb = fmaf(mu, o[e], x[e]);
-          if (in) buf[at + e * step] = nb;
-          w = nesterov ? fmaf(mu, nb, x[e]) : nb;
+          const float nb = fmaf(mu, o[q][e], w);
+          if (in) buf[r.at + e * r.step] = nb;
+          w = nesterov ? fmaf(mu, nb, w) : nb;
         }
         w = in ? w : 0.f;
         s = fma(static_cast<double>(w), static_cast<double>(w), s);
@@ -957,9 +992,8 @@ __global__ __launch_bounds__(kSmallThreads, 1) void ns_small_kernel(NsItems its,
   const NsTarget tg{nullptr, 0.f, 0.f, sc.small};
 #pragma unroll
   for (int q = 0; q < kRuns; ++q) {
-    const int id = static_cast<int>(threadIdx.x) + q * kSmallThreads;
-    if (id < runs) {
-      const int kc = place[q] >> 6, i = place[q] & 63;
+    const SmRun r = run_of(q);
+    if (r.on) {
       f16x8 hi, lo;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -967,7 +1001,7 @@ __global__ __launch_bounds__(kSmallThreads, 1) void ns_small_kernel(NsItems its,
         hi[e] = p.hi;
         lo[e] = p.lo;
       }
-      const unsigned at = sm_at(X, xp, i, chunk_of(8 * kc));
+      const unsigned at = sm_at(X, xp, r.i, chunk_of(8 * r.kc));
       *lds_ptr<lds_f16x8>(at) = hi;
       *lds_ptr<lds_f16x8>(at ^ 64) = lo;
     }
@@ -975,17 +1009,21 @@ __global__ __launch_bounds__(kSmallThreads, 1) void ns_small_kernel(NsItems its,
   __syncthreads();
 
   const int bi = 32 * (wave & 1), bc = 32 * ((wave >> 1) & 1), part = wave >> 2;
+  const SmBlock bl = sm_block(wave);
   for (int p = 0, step = 0; p < pl.nphase; ++p) {
-    {  // A = X X^T, a 32 x 32 block and every second 16 k a wave; the halves meet in MT
+    {  // A = X X^T, a 32 x 32 block and every third 16 k a wave; the thirds meet in MT and MP
       f32x16 acc = zero16(), cross = zero16();
-      for (int st = part; st < np / 16; st += 2) {
+      const int ln = anew(lane);
+      for (int st = part; st < np / 16; st += 3) {
         f16x8 lf[2], rf[2];
-        sm_rows(lf, X, xp, bi, st, lane);
-        sm_rows(rf, X, xp, bc, st, lane);
+        sm_rows(lf, X, xp, bi, st, ln);
+        sm_rows(rf, X, xp, bc, st, ln);
         mma_pairs(acc, cross, lf, rf);
       }
-      lds_f32* sum = lds_ptr<lds_f32>(MT) + (wave & 3) * 1024 + lane;
+      const int mine = (wave & 3) * 1024 + lane;
+      const lds_f32 *sum1 = lds_ptr<lds_f32>(MT) + mine, *sum2 = lds_ptr<lds_f32>(MP) + mine;
       if (part) {
+        lds_f32* sum = lds_ptr<lds_f32>(part == 1 ? MT : MP) + mine;
 #pragma unroll
         for (int r = 0; r < 16; ++r) sum[64 * r] = acc[r] + cross[r];
       }
@@ -996,10 +1034,10 @@ __global__ __launch_bounds__(kSmallThreads, 1) void ns_small_kernel(NsItems its,
 #pragma unroll
           for (int q = 0; q < 4; ++q) {  // four rows of a column: the mirror image's four columns of a row
             f16x4 hi, lo;
-            const int row = bi + 8 * q + 4 * h, col = bc + j;
+            const int row = bi + 8 * q + 4 * (ln >> 5), col = bc + (ln & 31);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const Pair pr = split_pair(((acc[4 * q + e] + cross[4 * q + e]) + sum[64 * (4 * q + e)]) * mul);
+              const Pair pr = split_pair((((acc[4 * q + e] + cross[4 * q + e]) + sum1[64 * (4 * q + e)]) + sum2[64 * (4 * q + e)]) * mul);
               hi[e] = pr.hi;
               lo[e] = pr.lo;
               const unsigned at = sm_at(MA, 256, row + e, chunk_of(col)) + static_cast<unsigned>(2 * (col & 7));
@@ -1021,42 +1059,33 @@ __global__ __launch_bounds__(kSmallThreads, 1) void ns_small_kernel(NsItems its,
       const float sp = pl.sp[step];
       const bool more = i + 1 < pl.phases[p];
       const unsigned P = i == 0 ? MQ : MP;  // the first P is Q
-      f32x4 v[2], vq[2];
-      sm_square(MA, MA, 1.f / (kScale * kScale), v, wave, lane);
-      {
+      f32x4 v, vq;
+      if (bl.on) {
+        v = sm_square(MA, MA, 1.f / (kScale * kScale), bl, lane);
         const int ln = anew(lane);
+        const unsigned at = sm_mirror(MA, bl, ln);
+        const f16x4 ah = *lds_ptr<lds_f16x4>(at), al = *lds_ptr<lds_f16x4>(at ^ 64);
 #pragma unroll
-        for (int turn = 0; turn < 2; ++turn) {
-          const SmBlock bl = sm_block(wave, turn);
-          if (!bl.on) continue;
-          const unsigned at = sm_mirror(MA, bl, ln);
-          const f16x4 ah = *lds_ptr<lds_f16x4>(at), al = *lds_ptr<lds_f16x4>(at ^ 64);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = (static_cast<float>(ah[e]) + static_cast<float>(al[e])) * (1.f / kScale);
-            v[turn][e] = fmaf(pl.c, v[turn][e], pl.b * x);
-            if (bl.r0 + 4 * (ln >> 4) + e == bl.c0 + (ln & 15)) v[turn][e] += pl.a;
-            v[turn][e] *= sp;
-          }
+        for (int e = 0; e < 4; ++e) {
+          const float x = (static_cast<float>(ah[e]) + static_cast<float>(al[e])) * (1.f / kScale);
+          v[e] = fmaf(pl.c, v[e], pl.b * x);
+          if (bl.r0 + 4 * (ln >> 4) + e == bl.c0 + (ln & 15)) v[e] += pl.a;
+          v[e] *= sp;
         }
-      }
-      sm_put(P, v, wave, lane);
-      __syncthreads();
-      if (more) {  // T = P A
-        sm_square(P, MA, 1.f / sp, v, wave, lane);
-        sm_put(MT, v, wave, lane);
-      }
-      if (i > 0) {  // Q <- P Q, stored once every wave has read Q
-        sm_square(P, MQ, pl.sq[step] / (sp * sq), vq, wave, lane);
-        sq = pl.sq[step];
-      } else {
-        sq = sp;
+        sm_put(P, v, bl, lane);
       }
       __syncthreads();
-      if (i > 0) sm_put(MQ, vq, wave, lane);
-      if (more) {  // A <- T P (at the first step P is Q, which no wave stores then)
-        sm_square(MT, P, 1.f / sp, v, wave, lane);
-        sm_put(MA, v, wave, lane);
+      if (bl.on && more) {  // T = P A
+        v = sm_square(P, MA, 1.f / sp, bl, lane);
+        sm_put(MT, v, bl, lane);
+      }
+      if (bl.on && i > 0) vq = sm_square(P, MQ, pl.sq[step] / (sp * sq), bl, lane);  // Q <- P Q, stored once every wave has read Q
+      sq = i > 0 ? pl.sq[step] : sp;
+      __syncthreads();
+      if (bl.on && i > 0) sm_put(MQ, vq, bl, lane);
+      if (bl.on && more) {  // A <- T P (at the first step P is Q, which no wave stores then)
+        v = sm_square(MT, P, 1.f / sp, bl, lane);
+        sm_put(MA, v, bl, lane);
       }
       __syncthreads();
     }
@@ -1067,7 +1096,7 @@ __global__ __launch_bounds__(kSmallThreads, 1) void ns_small_kernel(NsItems its,
       f32x16 acc[2], cross[2];
 #pragma unroll
       for (int b = 0; b < 2; ++b) acc[b] = cross[b] = zero16();
-      const int ln = anew(lane);
+      const int ln = anew(lane), j = ln & 31, h = ln >> 5;
 #pragma unroll
       for (int st = 0; st < 4; ++st) {
         f16x8 xf[2], qf[2];

@@ -157,6 +157,16 @@ def test_batches_and_strides(device):
             check(out[i], view[i])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("start,apart", [(0, 40 * 64), (0, 40 * 64 + 8), (0, 40 * 64 + 4), (1, 40 * 64 + 3)])
+def test_rows_of_any_alignment(device, dtype, start, apart):
+    from protoseg_amd import optim
+    flat = torch.zeros(start + 2 * apart + 40 * 64, dtype=dtype, device=device)
+    g = flat.as_strided((3, 40, 64), (apart, 64, 1), start)
+    g.copy_(matrix((3, 40, 64), 25).to(dtype))
+    check_batch(optim.orthogonalize(g), g)
+
+
 def test_matrices_do_not_touch_each_other(device):
     from protoseg_amd import optim
     g = matrix((5, 48, 80), 6).to(device)
