@@ -9,7 +9,6 @@ HIP calls to that same runtime, so stream handles from ``torch.cuda`` are valid 
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 import pathlib
@@ -165,12 +164,15 @@ def stream_of(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
-_HERE = contextlib.nullcontext()
-
-
-def on_device(device: torch.device):
-    """``torch.cuda.device(device)``, without its cost where the device is the current one already."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def call_on(index: int, name: str, *args) -> None:
+    """``call(name, *args, stream)`` on device ``index`` and its current stream (a plain integer: no object but the
+    arguments' is made, which counts where an operator's kernels are shorter than its call)."""
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return call_on(index, name, *args)
+    status = getattr(_handle or load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status != OK:
+        check(name, status)
 
 
 def require_device(*tensors: torch.Tensor) -> torch.device:

@@ -22,95 +22,105 @@ import torch.nn as nn
 from torch import Tensor
 
 from . import _lib
-from .ops import _x_dtype
 
 ACTIVATIONS = {"identity": 0, "relu": 1, "sigmoid": 2, "silu": 3}
 
 
-def _rows(x: Tensor) -> Tuple[Tensor, int, int]:
-    """x as the kernels read it, channel stride 1 and one stride from pixel to pixel, with its sample
-    and pixel strides. A channels-last map, and a slice of one along batch or channels, passes as it
-    is; anything else is copied. A stride that is never stepped over is given its dense value."""
-    B, C, H, W = x.shape
-    sb, sc, sh, sw = x.stride()
+# Beside its kernels a training call on the backbone's maps is host time, most of it Python objects that the
+# autograd thread and the caller's take from each other's caches. So what types, shapes and strides decide is
+# worked out once for each of them, and a call looks it up.
+@functools.lru_cache(maxsize=4096)
+def _strides(shape: torch.Size, stride: Tuple[int, ...]) -> Optional[Tuple[int, int]]:
+    """Sample and pixel stride of a map as the kernels read it, channel stride 1 and one stride from pixel to
+    pixel: a channels-last map, and a slice of one along batch or channels. None: anything else, which is
+    copied. A stride that is never stepped over is given its dense value."""
+    B, C, H, W = shape
+    sb, sc, sh, sw = stride
     sp = sw if W > 1 else sh if H > 1 else C
     if (sc == 1 or C == 1) and sp >= C and (H == 1 or W == 1 or sh == sw * W):
         if B == 1:
-            return x, H * W * sp, sp
+            return H * W * sp, sp
         if sb >= sp * (H * W - 1) + C:
-            return x, sb, sp
+            return sb, sp
+    return None
+
+
+def _rows(x: Tensor) -> Tuple[Tensor, int, int]:
+    """x, or its channels-last copy, and its strides."""
+    at = _strides(x.shape, x.stride())
+    if at is not None:
+        return (x, *at)
+    B, C, H, W = x.shape
     return x.contiguous(memory_format=torch.channels_last), H * W * C, C
 
 
-@functools.lru_cache(maxsize=1024)
-def _workspace_bytes(code: int, B: int, HW: int, C: int, groups: int, backward: int) -> int:
-    return _lib.load().protoseg_group_norm_workspace_size(code, B, HW, C, groups, backward)
+_CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
-def _empty_like_map(x: Tensor) -> Tensor:
-    return torch.empty(x.shape, dtype=x.dtype, device=x.device, memory_format=torch.channels_last)
-
-
-def _check(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], act: int) -> int:
-    """Refuses what the kernels do not take; x's dtype code."""
-    if x.dim() != 4:
-        raise _lib.ProtosegError(f"group norm takes [B, C, H, W] maps; got {tuple(x.shape)}")
-    code = _x_dtype(x)
-    C = x.shape[1]
+@functools.lru_cache(maxsize=4096)
+def _sizes(dtype: torch.dtype, shape: torch.Size, groups: int) -> Tuple[Tuple[int, int, int, int], int, int]:
+    """(dtype code, B, HW, C) and the workspace bytes of a forward and of a backward. Refuses what the kernels do
+    not take."""
+    if len(shape) != 4:
+        raise _lib.ProtosegError(f"group norm takes [B, C, H, W] maps; got {tuple(shape)}")
+    if dtype not in _CODES:
+        raise _lib.ProtosegError(f"feature map dtype {dtype} unsupported (float32, bfloat16 or float16)")
+    B, C, H, W = shape
     if groups < 1 or C < 1 or C % groups:
         raise _lib.ProtosegError(f"{C} channels do not divide into {groups} groups")
-    if weight is not None and (weight.dtype != torch.float32 or weight.shape != (C,)):
-        raise _lib.ProtosegError(f"group norm weight: float32 [{C}] expected, got {weight.dtype} {tuple(weight.shape)}")
-    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (C,)):
-        raise _lib.ProtosegError(f"group norm bias: float32 [{C}] expected, got {bias.dtype} {tuple(bias.shape)}")
-    if act not in ACTIVATIONS.values():
-        raise _lib.ProtosegError(f"activation code {act} unknown")
-    return code
+    sizes = (_CODES[dtype], B, H * W, C)
+    nbytes = _lib.load().protoseg_group_norm_workspace_size
+    return sizes, nbytes(*sizes, groups, 0), nbytes(*sizes, groups, 1)
+
+
+def _check_affine(name: str, t: Optional[Tensor], C: int, index: int) -> Optional[Tensor]:
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.shape != (C,):
+        raise _lib.ProtosegError(f"group norm {name}: float32 [{C}] expected, got {t.dtype} {tuple(t.shape)}")
+    if t.get_device() != index:
+        raise _lib.ProtosegError(f"group norm {name} on {t.device}: the map's device expected")
+    return t.contiguous()
 
 
 def _forward(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], groups: int, eps: float, act: int):
     """y, stats and what a backward needs again: (x, weight, bias as read; the call's sizes)."""
-    code = _check(x, groups, weight, bias, act)
-    dev = _lib.require_device(x, weight, bias)
-    x, sb, sp = _rows(x)
-    weight = weight.contiguous() if weight is not None else None
-    bias = bias.contiguous() if bias is not None else None
-    B, C, H, W = x.shape
-    y = _empty_like_map(x)
-    stats = torch.empty((B, groups, 2), device=dev, dtype=torch.float64)
-    sizes = (code, B, H * W, C, sb, sp)
-    if x.numel() == 0:
+    plan = _sizes(x.dtype, x.shape, groups)
+    sizes, nbytes = plan[0], plan[1]
+    if not 0 <= act < len(ACTIVATIONS):
+        raise _lib.ProtosegError(f"activation code {act} unknown")
+    index = x.get_device()
+    weight, bias = _check_affine("weight", weight, sizes[3], index), _check_affine("bias", bias, sizes[3], index)
+    if index < 0:
+        _lib.require_device(x)  # refuses
+    x, *at = _rows(x)
+    y = torch.empty_like(x, memory_format=torch.channels_last)
+    stats = x.new_empty((sizes[1], groups, 2), dtype=torch.float64)
+    if sizes[1] == 0 or sizes[2] == 0:
         stats.zero_()
     else:
-        lib = _lib.load()
-        with _lib.on_device(dev):
-            nbytes = _workspace_bytes(code, B, H * W, C, groups, 0)
-            ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-            _lib.check("protoseg_group_norm_fwd", lib.protoseg_group_norm_fwd(
-                x.data_ptr(), *sizes, groups, _lib.addr(weight), _lib.addr(bias), eps, act, y.data_ptr(), stats.data_ptr(),
-                ws.data_ptr(), nbytes, _lib.stream_of(dev)))
-    return y, stats, (x, weight, bias), sizes
+        ws = x.new_empty(nbytes, dtype=torch.uint8)
+        _lib.call_on(index, "protoseg_group_norm_fwd", x.data_ptr(), *sizes, *at, groups, _lib.addr(weight),
+                     _lib.addr(bias), eps, act, y.data_ptr(), stats.data_ptr(), ws.data_ptr(), nbytes)
+    return y, stats, (x, weight, bias), (plan, at)
 
 
-def _backward(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], stats: Tensor, sizes, g_y: Tensor, groups: int,
+def _backward(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], stats: Tensor, plan, g_y: Tensor, groups: int,
               act: int, need_x: bool, need_weight: bool, need_bias: bool):
     """The backward on tensors that _forward returned; only g_y is new to it."""
-    dev = x.device
-    g_y, gsb, gsp = _rows(g_y if g_y.dtype == x.dtype else g_y.to(x.dtype))
+    (sizes, _, nbytes), at = plan
     C = sizes[3]
-    g_x = _empty_like_map(x) if need_x else None
-    if x.numel() == 0:
+    g_x = torch.empty_like(x, memory_format=torch.channels_last) if need_x else None
+    if sizes[1] == 0 or sizes[2] == 0:
         zero = x.new_zeros(C, dtype=torch.float32)
         return g_x, zero if need_weight else None, zero.clone() if need_bias else None
-    g_w = torch.empty(C, device=dev, dtype=torch.float32) if need_weight else None
-    g_b = torch.empty(C, device=dev, dtype=torch.float32) if need_bias else None
-    lib = _lib.load()
-    with _lib.on_device(dev):
-        nbytes = _workspace_bytes(*sizes[:4], groups, 1)
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-        _lib.check("protoseg_group_norm_bwd", lib.protoseg_group_norm_bwd(
-            x.data_ptr(), g_y.data_ptr(), *sizes, gsb, gsp, groups, _lib.addr(weight), _lib.addr(bias), act,
-            stats.data_ptr(), _lib.addr(g_x), _lib.addr(g_w), _lib.addr(g_b), ws.data_ptr(), nbytes, _lib.stream_of(dev)))
+    g_y, *g_at = _rows(g_y if g_y.dtype == x.dtype else g_y.to(x.dtype))
+    g_w = x.new_empty(C, dtype=torch.float32) if need_weight else None
+    g_b = x.new_empty(C, dtype=torch.float32) if need_bias else None
+    ws = x.new_empty(nbytes, dtype=torch.uint8)
+    _lib.call_on(x.get_device(), "protoseg_group_norm_bwd", x.data_ptr(), g_y.data_ptr(), *sizes, *at, *g_at, groups,
+                 _lib.addr(weight), _lib.addr(bias), act, stats.data_ptr(), _lib.addr(g_x), _lib.addr(g_w), _lib.addr(g_b),
+                 ws.data_ptr(), nbytes)
     return g_x, g_w, g_b
 
 
@@ -124,14 +134,16 @@ def group_norm_backward(x: Tensor, g_y: Tensor, weight: Optional[Tensor], bias: 
                         act: int, need_x: bool = True, need_weight: bool = True,
                         need_bias: bool = True) -> Tuple[Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
     """Gradients of group_norm_forward's y with respect to (x, weight, bias); None where not needed."""
-    code = _check(x, groups, weight, bias, act)
+    plan = _sizes(x.dtype, x.shape, groups)
+    C = plan[0][3]
+    if not 0 <= act < len(ACTIVATIONS):
+        raise _lib.ProtosegError(f"activation code {act} unknown")
     _lib.require_device(x, g_y, weight, bias, stats)
     if g_y.shape != x.shape or stats.dtype != torch.float64 or tuple(stats.shape) != (x.shape[0], groups, 2):
         raise _lib.ProtosegError("group norm backward: g_y and stats must be of the forward's shapes")
-    x, sb, sp = _rows(x)
-    B, C, H, W = x.shape
-    return _backward(x, weight.contiguous() if weight is not None else None, bias.contiguous() if bias is not None else None,
-                     stats.contiguous(), (code, B, H * W, C, sb, sp), g_y, groups, act, need_x, need_weight, need_bias)
+    weight, bias = _check_affine("weight", weight, C, x.get_device()), _check_affine("bias", bias, C, x.get_device())
+    x, *at = _rows(x)
+    return _backward(x, weight, bias, stats.contiguous(), (plan, at), g_y, groups, act, need_x, need_weight, need_bias)
 
 
 class _GroupNorm(torch.autograd.Function):
@@ -139,16 +151,18 @@ class _GroupNorm(torch.autograd.Function):
     # host time than the kernels take on the backbone's maps at the micro-batch of 2
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act):
-        y, stats, used, ctx.sizes = _forward(x, weight, bias, groups, eps, act)
+        y, stats, used, plan = _forward(x, weight, bias, groups, eps, act)
         ctx.save_for_backward(*used, stats)
-        ctx.groups, ctx.act = groups, act
+        ctx.call = plan, groups, act
         return y
 
     @staticmethod
     def backward(ctx, g_y):
         if torch.is_grad_enabled():  # create_graph
             raise _lib.ProtosegError("group norm has no second derivative")
-        return (*_backward(*ctx.saved_tensors, ctx.sizes, g_y, ctx.groups, ctx.act, *ctx.needs_input_grad[:3]), None, None, None)
+        plan, groups, act = ctx.call
+        need = ctx.needs_input_grad
+        return (*_backward(*ctx.saved_tensors, plan, g_y, groups, act, need[0], need[1], need[2]), None, None, None)
 
 
 def group_norm(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5,

@@ -205,12 +205,10 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS,
         m = m.contiguous()
     stride = m.stride(0) if count > 1 else rows * cols
     lib = _lib.load()
-    with _lib.on_device(dev):
-        nbytes = lib.protoseg_orthogonalize_workspace_size(count, rows, cols)
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-        _lib.check("protoseg_orthogonalize", lib.protoseg_orthogonalize(
-            m.data_ptr(), code, count, rows, cols, stride, int(steps), a, b, c, float(eps), out.data_ptr(), ws.data_ptr(),
-            nbytes, _lib.stream_of(dev)))
+    nbytes = lib.protoseg_orthogonalize_workspace_size(count, rows, cols)
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    _lib.call_on(dev.index, "protoseg_orthogonalize", m.data_ptr(), code, count, rows, cols, stride, int(steps), a, b, c,
+                 float(eps), out.data_ptr(), ws.data_ptr(), nbytes)
     return out
 
 
@@ -234,10 +232,15 @@ class Muon(torch.optim.Optimizer):
             raise ValueError("invalid Muon hyper-parameters")
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
                                       ns_steps=ns_steps, ns_coefficients=tuple(ns_coefficients), eps=eps, scale=scale))
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.dim() < 2:
-                    raise ValueError(f"Muon takes matrices; got a parameter of shape {tuple(p.shape)}")
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        params = self.param_groups[-1]["params"]
+        small = [tuple(p.shape) for p in params if p.dim() < 2]
+        if small or len(set(map(id, params))) < len(params):
+            self.param_groups.pop()
+            raise ValueError(f"Muon takes matrices; got a parameter of shape {small[0]}" if small else
+                             "Muon: a parameter is in the group twice")  # its updates would race in one launch
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -280,13 +283,12 @@ class Muon(torch.optim.Optimizer):
             addr = [ctypes.cast(a, ctypes.c_void_p) for a in arrays]
             a, b, c = (float(v) for v in group["ns_coefficients"])
             lib = _lib.load()
-            with _lib.on_device(dev):
-                nbytes = lib.protoseg_muon_workspace_size(k, addr[3], addr[4])
-                ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-                _lib.check("protoseg_muon_step", lib.protoseg_muon_step(
-                    k, *addr, float(group["momentum"]), int(bool(group["nesterov"])), float(group["lr"]),
-                    float(group["weight_decay"]), _MUON_SCALES[group["scale"]], int(group["ns_steps"]), a, b, c,
-                    float(group["eps"]), ws.data_ptr(), nbytes, _lib.stream_of(dev)))
+            nbytes = lib.protoseg_muon_workspace_size(k, addr[3], addr[4])
+            ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+            _lib.call_on(dev.index, "protoseg_muon_step", k, *addr, float(group["momentum"]), int(bool(group["nesterov"])),
+                         float(group["lr"]), float(group["weight_decay"]), _MUON_SCALES[group["scale"]],
+                         int(group["ns_steps"]), a, b, c, float(group["eps"]), ws.data_ptr(), nbytes)
+            torch.autograd.graph.increment_version(ps)  # as an in-place operation of torch's does
         return loss
 
 

@@ -350,3 +350,16 @@ def test_two_streams_at_once_and_same_bits(device):
     torch.cuda.synchronize()
     for k, o in enumerate(got):
         assert torch.equal(o, want[k % 2])
+
+
+def test_a_step_is_seen_by_autograd(device):
+    """Parameters are changed in place: a graph that saved their old values refuses its backward."""
+    from protoseg_amd import optim
+    p = torch.nn.Parameter(matrix((20, 30), 41).to(device))
+    x = torch.ones(30, device=device, requires_grad=True)
+    opt = optim.Muon([p])
+    y = (p * p) @ x
+    p.grad = torch.ones_like(p)
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()

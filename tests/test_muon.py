@@ -91,3 +91,18 @@ def test_which_layouts_are_rows():
     assert not optim._dense_rows(torch.zeros(6, 4).t())
     assert not optim._dense_rows(torch.zeros(4, 8)[:, ::2])
     assert not optim._dense_rows(torch.zeros(8, 4)[::2])
+
+
+def test_a_group_is_checked_as_it_is_added():
+    from protoseg_amd import optim
+    p, q = torch.nn.Parameter(torch.zeros(4, 3)), torch.nn.Parameter(torch.zeros(2, 5))
+    opt = optim.Muon([p])
+    with pytest.warns(UserWarning), pytest.raises(ValueError, match="twice"):
+        opt.add_param_group({"params": [q, q]})
+    with pytest.raises(ValueError, match=r"\(7,\)"):
+        opt.add_param_group({"params": [q, torch.nn.Parameter(torch.zeros(7))]})
+    with pytest.raises(ValueError):
+        opt.add_param_group({"params": p})
+    assert len(opt.param_groups) == 1
+    opt.add_param_group({"params": q, "lr": 0.5})
+    assert [g["lr"] for g in opt.param_groups] == [2e-2, 0.5]
