@@ -22,8 +22,8 @@ namespace protoseg {
 namespace {
 
 constexpr int kGnThreads = 256;
-constexpr long long kGnTarget = 1024, kGnLeast = 16384;  // gn_chunks
-constexpr long long kGnJoinInside = 4096;                // gn_apply_kernel
+constexpr long long kGnTarget = 512, kGnLeast = 4096, kGnEnough = 16384;  // gn_chunks
+constexpr long long kGnJoinInside = 4096;                               // gn_apply_kernel
 
 enum GnAct { kGnIdentity = 0, kGnRelu = 1, kGnSigmoid = 2, kGnSilu = 3 };
 
@@ -370,7 +370,7 @@ __device__ __forceinline__ float grad_z(float gy, float x, float d, float a, flo
 
 // Partial sums of one chunk, S1 = sum gz and S2 = sum gz xh: per channel (part, f32 rows [2][C] of
 // each workgroup), and weighted by w over each group (gpart). f32 inside a chunk, where a thread adds up
-// ppc / R values of mixed sign (8 to 34 in this library's maps; more where a large batch leaves one chunk a
+// ppc / R values of mixed sign (8 to 67 in this library's maps; more where a large batch leaves one chunk a
 // sample); the chunks are joined in f64. 32 x 64 x 65 x 65 f32: 16.1 us, 4.3 TB/s.
 template <typename T, int V, int S, int ACT>
 __global__ __launch_bounds__(kGnThreads) void gn_bwd_sums_kernel(GnMap x, GnMap gy, GnShape s, GnParts pt,
@@ -593,14 +593,16 @@ __global__ void gn_zero_kernel(float* a, float* b, int n) {
   }
 }
 
-// Chunks per sample, the same in both passes over a map: a chunk's second pass runs on the XCD of its
-// first (workgroup i on XCD i % 8) and finds it in that XCD's L2 where the map is below 8 x 4 MiB.
-// About 1024 workgroups over the samples, none below 16384 elements (its launch, its constants and
-// its joining would cost more than its share of the map).
+// Chunks per sample, the same in both passes over a map. About 512 workgroups over the samples (1024: 1 x 2048 x
+// 129 x 257 bf16 93.3 us for 91.5, forward and backward of 32 x 64 x 65 x 65 f32 63.0 us for 58.8; 256: 2 x 64 x
+// 257 x 257 bf16 50.2 us for 45.5), none below 4096 elements (3 x 150 x 33 x 47 f16: 20.4 us, with 16384
+// 29.7). Where every workgroup of the second pass would join more than 2048 pairs of a sample, shorter chunks cost
+// as much as they save: 16384 elements then (2 x 256 x 65 x 65 bf16: 34.2 us, with 4096 37.1).
 void gn_chunks(GnShape& s) {
   long long want = ceil_div(kGnTarget, s.B);
-  const long long most = ceil_div(static_cast<long long>(s.HW) * s.C, kGnLeast);
-  if (want > most) want = most;
+  const long long all = static_cast<long long>(s.HW) * s.C, inside = kGnJoinInside / 2 / s.G, enough = ceil_div(all, kGnEnough);
+  if (want > ceil_div(all, kGnLeast)) want = ceil_div(all, kGnLeast);
+  if (want > inside && want > enough) want = inside > enough ? inside : enough;
   if (want > s.HW) want = s.HW;
   if (want < 1) want = 1;
   s.ppc = static_cast<int>(ceil_div(s.HW, want));
