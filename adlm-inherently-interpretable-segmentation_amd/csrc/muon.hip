@@ -274,7 +274,7 @@ __device__ __forceinline__ NsScale scale_of(double squares, float eps) {
 }
 
 // X0 of one 64 x 64 tile: the (update's) values over their norm, transposed where the matrix is tall, as
-// f16 pairs, zeros in the padding. 104 us for 47e6 elements: 5.4 TB/s, the reads from the last-level cache.
+// f16 pairs, zeros in the padding. 102 us for 47e6 elements: 5.5 TB/s, the reads from the last-level cache.
 template <typename T, bool STEP>
 __global__ __launch_bounds__(256) void ns_load_kernel(NsGroups gs, NsItems its, float mu, int nesterov, float eps) {
   __shared__ float tile[64][65];
@@ -382,8 +382,8 @@ __device__ __forceinline__ void stage_wait(int later) {
 
 // T x T output tile, 4 waves of (T / 2) x (T / 2), 3 MFMAs per 32 x 32 x 16 block. LDS-DMA fills a ring of
 // stages of 32 k, ring_of - 1 ahead of the products, with one barrier a stage. In the step over a ResNet-101's
-// convolutions (109 matrices, 47e6 elements) the Gram product takes 113 us, Q X 145 us, Q X with the parameters'
-// update 182 us, a product of squares 31 us: 505, 662, 528 and 403 TFLOP/s of f16, where a large library product
+// convolutions (109 matrices, 47e6 elements) the Gram product takes 109 us, Q X 142 us, Q X with the parameters'
+// update 177 us, a product of squares 30 us: 524, 677, 545 and 410 TFLOP/s of f16, where a large library product
 // reaches 1100. LDS bounds a 64 x 64 tile: a stage is 192 cycles of MFMA on each SIMD, and 32 KiB read and 16 KiB
 // written at 128 B a cycle are 384. At 128 x 128 they are even (768 and 768), but the symmetric products would
 // compute a fifth more and leave half the chip's places empty at the end (measured slower).
@@ -727,7 +727,7 @@ __global__ __launch_bounds__(256, 1) void ns_thin_kernel(NsGroups gs, NsJobs js)
   }
 }
 
-// The partials of a split Gram product joined in a fixed order (8.2 us in the 109 matrices' step, bound by reading
+// The partials of a split Gram product joined in a fixed order (8.0 us in the 109 matrices' step, bound by reading
 // them): a workgroup takes one 32 x 32 block on or
 // above the diagonal, each wave every fourth split, and stores it with its mirror image.
 __global__ __launch_bounds__(256) void ns_join_kernel(NsGroups gs, float inv, int grown) {
@@ -1575,6 +1575,14 @@ extern "C" int protoseg_muon_step(int n_tensors, float* const* params, const flo
   for (int i = 0; i < n_tensors; ++i)
     if (rows[i] && cols[i] && (!params[i] || !grads[i] || !momentum_bufs[i]))
       return fail(PROTOSEG_ERR_INVALID, "muon tensor %d: null pointer", i);
+  for (float* const* list : {params, momentum_bufs}) {  // twice in the call, two workgroups would write it at once
+    std::vector<const float*> seen;
+    for (int i = 0; i < n_tensors; ++i)
+      if (rows[i] && cols[i]) seen.push_back(list[i]);
+    std::sort(seen.begin(), seen.end());
+    if (std::adjacent_find(seen.begin(), seen.end()) != seen.end())
+      return fail(PROTOSEG_ERR_INVALID, "muon: a parameter or momentum buffer is in the call twice");
+  }
   for (const MuonRun& r : runs) {
     NsGroups gs;
     const size_t n = ns_layout(gs, r.mats, nullptr, nullptr);

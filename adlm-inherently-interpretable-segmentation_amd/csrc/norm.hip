@@ -157,8 +157,8 @@ __device__ __forceinline__ void pair_total(const P2* __restrict__ part, const Gn
 // Partial sums of one chunk: (sum x, sum x^2) of each group that the workgroup's channels meet.
 // f64 from the first addition: the variance is a difference of the two, and sums of exact input
 // values keep it right for means up to 2^20 spreads; two f64 operations an element are far below
-// the rate that would bound the kernel. 1 x 2048 x 129 x 257 bf16: 22.6 us, 6.0 TB/s. Maps of a few MB
-// (2 x 256 x 65 x 65 bf16: 6.1 us) are a launch and the latency of two rounds of loads.
+// the rate that would bound the kernel. 1 x 2048 x 129 x 257 bf16: 21.6 us, 6.3 TB/s. Maps of a few MB
+// (2 x 256 x 65 x 65 bf16: 4.3 us) are a launch and the latency of two rounds of loads.
 template <typename T, int V, int S>
 __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(GnMap x, GnShape s, GnParts pt, double2* __restrict__ part) {
   constexpr int kN = V / S, kU = 8;
@@ -286,8 +286,8 @@ __device__ __forceinline__ void load_coef(GnCoef<V, S>& k, const float4* cg, con
 // y = act(z). part: the statistics' partials, joined here by every workgroup (the first chunk's
 // leave them in `stat`), or null where gn_join_kernel has joined them: a launch less costs more
 // than a few thousand pairs read from L2 by each workgroup, many more than that do not.
-// 1 x 2048 x 129 x 257 bf16: 44.8 us, 6.1 TB/s read and written (56.7 without the next rows' loads in
-// flight while these are computed); 2 x 256 x 65 x 65 bf16: 9.4 us.
+// 1 x 2048 x 129 x 257 bf16: 44.6 us, 6.1 TB/s read and written (56.7 without the next rows' loads in
+// flight while these are computed); 2 x 256 x 65 x 65 bf16: 9.3 us.
 template <typename T, int V, int S, int ACT>
 __global__ __launch_bounds__(kGnThreads) void gn_apply_kernel(GnMap x, GnShape s, GnParts pt, const double2* __restrict__ part,
                                                               double eps, double2* __restrict__ stat,
@@ -371,7 +371,7 @@ __device__ __forceinline__ float grad_z(float gy, float x, float d, float a, flo
 // Partial sums of one chunk, S1 = sum gz and S2 = sum gz xh: per channel (part, f32 rows [2][C] of
 // each workgroup), and weighted by w over each group (gpart). f32 inside a chunk, where a thread adds up
 // ppc / R values of mixed sign (8 to 67 in this library's maps; more where a large batch leaves one chunk a
-// sample); the chunks are joined in f64. 32 x 64 x 65 x 65 f32: 16.1 us, 4.3 TB/s.
+// sample); the chunks are joined in f64. 32 x 64 x 65 x 65 f32: 14.7 us, 4.7 TB/s.
 template <typename T, int V, int S, int ACT>
 __global__ __launch_bounds__(kGnThreads) void gn_bwd_sums_kernel(GnMap x, GnMap gy, GnShape s, GnParts pt,
                                                                  const double2* __restrict__ stat,
@@ -473,7 +473,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_sums_kernel(GnMap x, GnMap 
 // g_x; and in the first `nsum` workgroups the sums of the channels' partials over chunks and
 // samples (g_w, g_beta), 16 channels x 16 lanes each, so that their chain of loads runs beside the
 // map's. Either part may be absent. gpart / gsum: the groups' partials, or joined (gn_join_kernel).
-// 32 x 64 x 65 x 65 f32: 19.9 us, 5.2 TB/s.
+// 32 x 64 x 65 x 65 f32: 18.1 us, 5.7 TB/s.
 template <typename T, int V, int S, int ACT>
 __global__ __launch_bounds__(kGnThreads) void gn_bwd_apply_kernel(GnMap x, GnMap gy, GnShape s, GnParts pt, int nsum,
                                                                   const double2* __restrict__ stat,

@@ -222,7 +222,8 @@ class Muon(torch.optim.Optimizer):
     prototype vectors [P, C, 1, 1]. ``scale``: "original", s = sqrt(max(1, rows / cols)), or "rms",
     s = 0.2 sqrt(max(rows, cols)) (the update's root mean square then is about Adam's). Biases and other vectors belong to
     ``Adam``; ``train.PatchClassificationStep`` steps a list of optimizers. All tensors of a group share
-    the launches, and a HIP graph holding ``step()`` replays as successive steps. float32 on the GPU only.
+    the launches, and a HIP graph holding ``step()`` replays as successive steps (after one step outside of it,
+    which makes the momentum). float32 on the GPU only.
     """
 
     def __init__(self, params: Iterable, lr: float = 2e-2, momentum: float = 0.95, nesterov: bool = True,
@@ -259,6 +260,8 @@ class Muon(torch.optim.Optimizer):
                     raise _lib.ProtosegError("protoseg Muon: float32 matrices and dense gradients only")
                 st = self.state[p]
                 if "momentum_buffer" not in st:
+                    if p.is_cuda and torch.cuda.is_current_stream_capturing():  # every replay would zero it again
+                        raise _lib.ProtosegError("protoseg Muon: a captured step needs one step before it")
                     st["momentum_buffer"] = torch.zeros_like(p)
                 buf, g = st["momentum_buffer"], p.grad
                 if not _dense_rows(p):

@@ -363,3 +363,16 @@ def test_a_step_is_seen_by_autograd(device):
     opt.step()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+def test_a_first_step_is_not_captured(device):
+    from protoseg_amd import _lib, optim
+    p = torch.nn.Parameter(matrix((20, 30), 42).to(device))
+    p.grad = torch.ones_like(p)
+    opt = optim.Muon([p])
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(_lib.ProtosegError, match="one step before"):
+        with torch.cuda.graph(graph):
+            p.grad.add_(0)
+            opt.step()
+    opt.step()

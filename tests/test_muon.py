@@ -106,3 +106,13 @@ def test_a_group_is_checked_as_it_is_added():
     assert len(opt.param_groups) == 1
     opt.add_param_group({"params": q, "lr": 0.5})
     assert [g["lr"] for g in opt.param_groups] == [2e-2, 0.5]
+
+
+def test_a_tensor_twice_in_a_call_is_refused():
+    lib = _lib.load()
+    size, other = (ctypes.c_int32 * 2)(100, 100), (ctypes.c_int32 * 2)(200, 200)
+    once, twice = (ctypes.c_void_p * 2)(4096, 8192), (ctypes.c_void_p * 2)(4096, 4096)
+    for params, bufs in ((twice, once), (once, twice)):
+        assert lib.protoseg_muon_step(2, params, once, bufs, size, other, 0.9, 1, 0.1, 0.0, 0, 5, *NS, 1e-7, NULL, 0,
+                                      NULL) == _lib.ERR_INVALID
+        assert b"twice" in lib.protoseg_last_error()
