@@ -45,10 +45,23 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
+typedef __attribute__((address_space(3))) f16x8 lds_f16x8;
+typedef __attribute__((address_space(3))) f16x4 lds_f16x4;
+typedef __attribute__((address_space(3))) _Float16 lds_f16;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) float lds_f32;
+template <typename P>
+__device__ __forceinline__ P* lds_ptr(unsigned at) {
+  return reinterpret_cast<P*>(static_cast<uintptr_t>(at));
+}
+
 constexpr int kPad = 64;
 constexpr int kMaxGroups = 24, kMaxItems = 32, kMaxSteps = 32;
 constexpr float kScale = 1024.f;  // of X, A and T: entries below 16 (checked) stay below 2^14
 constexpr long long kThinTiles = 256;  // ns_thin_kernel's tiles at most: it has one workgroup a CU (22 matrices of 256, 792 tiles: 303 us for 195)
+// Up to so many 64 x 64 tiles (one a CU), of contractions of 8 stages or more, the two halves of a contraction run
+// beside each other (one matrix of 1024 x 1024: 245 us for 275; 100 of 64 x 500, 2 stages: 119 us for 114).
+constexpr long long kHalvesTiles = 256, kHalvesStages = 8;
 constexpr long long kApplyTiles = 384;  // from so many 128 x 128 tiles of Q X on, they beat 64 x 64 ones (backbone: 1178 us for 1236)
 constexpr int kNormThreads = 256, kMaxChunks = 256;
 constexpr long long kNormLeast = 16384;  // elements per workgroup of the sums of squares
@@ -387,15 +400,18 @@ __device__ __forceinline__ void stage_wait(int later) {
 // reaches 1100. LDS bounds a 64 x 64 tile: a stage is 192 cycles of MFMA on each SIMD, and 32 KiB read and 16 KiB
 // written at 128 B a cycle are 384. At 128 x 128 they are even (768 and 768), but the symmetric products would
 // compute a fifth more and leave half the chip's places empty at the end (measured slower).
-template <int T, int MODE, int OUT>
-__global__ __launch_bounds__(256, 160 * 1024 / (ring_of(T) * stage_bytes(T))) void ns_product_kernel(NsGroups gs, NsJobs js) {
+// G = 2: a second set of 4 waves takes the second half of the stages and hands its sums over at the end.
+template <int T, int MODE, int OUT, int G = 1>
+__global__ __launch_bounds__(256 * G, 160 * 1024 / (G * ring_of(T) * stage_bytes(T))) void ns_product_kernel(NsGroups gs, NsJobs js) {
+  static_assert(G == 1 || (G == 2 && T == 64 && MODE == kSym), "sums are handed over as one block a wave");
   constexpr int MI = T / 64, kPieces = T / 32;  // 1-KiB DMA pieces per operand and wave
   constexpr int kOperand = T * 128;             // bytes of one operand of a stage
   constexpr int kStages = ring_of(T);
   constexpr bool KX = MODE != kSym;             // the right operand's k runs down its rows
   extern __shared__ __attribute__((aligned(16))) unsigned char sm[];
-  const unsigned S0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)sm));
-  const int lane = threadIdx.x & 63, wave = bf16l::wave_id(), j = lane & 31, h = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = bf16l::wave_id() & 3, half = G == 2 ? bf16l::wave_id() >> 2 : 0, j = lane & 31, h = lane >> 5;
+  const unsigned S0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)sm)) +
+                      static_cast<unsigned>(half * kStages * stage_bytes(T));
   const int gi = place_of(gs.first, blockIdx.x);
   const NsGroup& g = gs.g[gi];
   const int nt = (g.mp + T - 1) / T, nc = KX ? (g.np + T - 1) / T : nt;
@@ -425,7 +441,8 @@ __global__ __launch_bounds__(256, 160 * 1024 / (ring_of(T) * stage_bytes(T))) vo
   const _Float16* R = pairs_of(gs, g, job.r, mat);
   const unsigned lbytes = static_cast<unsigned>(4LL * g.mp * K), rbytes = KX ? static_cast<unsigned>(x_bytes(g)) : lbytes;
   const int nst_all = K / 32;
-  const int st0 = nst_all * z / splits, nst = nst_all * (z + 1) / splits - st0;
+  const int z0 = nst_all * z / splits, z1 = nst_all * (z + 1) / splits;
+  const int turns = (z1 - z0 + G - 1) / G, st0 = z0 + half * turns, nst = G == 2 && half ? z1 - st0 : turns;  // turns or one less
 
   const rsrc_t rl = make_rsrc(L, lbytes), rr = make_rsrc(R, rbytes);
   unsigned vol[kPieces], vor[kPieces];
@@ -462,11 +479,12 @@ __global__ __launch_bounds__(256, 160 * 1024 / (ring_of(T) * stage_bytes(T))) vo
     for (int b = 0; b < MI; ++b) acc[a][b] = cross[a][b] = zero16();
 
   for (int st = 0; st < kStages - 1 && st < nst; ++st) issue(st);
-  for (int st = 0; st < nst; ++st) {
+  for (int st = 0; st < turns; ++st) {
     // this stage has landed (what was issued after it may be in flight), and every read of the stage before
     // it has returned
     stage_wait<2 * kPieces, kStages - 2>(nst - 1 - st);
     if (st + kStages - 1 < nst) issue(st + kStages - 1);  // into the stage that every wave has read before this barrier
+    if (G == 2 && st >= nst) break;  // the barrier above was the last
     const unsigned sb = S0 + static_cast<unsigned>((st % kStages) * stage_bytes(T));
     f16x8 lf[2][MI][2], rf[2][MI][2];
     auto read_step = [&](int ks) __attribute__((always_inline)) {
@@ -526,6 +544,18 @@ __global__ __launch_bounds__(256, 160 * 1024 / (ring_of(T) * stage_bytes(T))) vo
   for (int a = 0; a < MI; ++a)
 #pragma unroll
     for (int b = 0; b < MI; ++b) acc[a][b] += cross[a][b];
+  if constexpr (G == 2) {
+    lds_f32* sums = lds_ptr<lds_f32>(S0 - static_cast<unsigned>(half * kStages * stage_bytes(T))) + wave * 1024 + lane;
+    __syncthreads();  // no stage is read any more
+    if (half) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sums[64 * r] = acc[0][0][r];
+    }
+    __syncthreads();
+    if (half) return;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[0][0][r] += sums[64 * r];
+  }
 
 #pragma unroll
   for (int a = 0; a < MI; ++a)
@@ -787,16 +817,6 @@ struct NsPlan {
   float sp[kMaxSteps], sq[kMaxSteps];  // scales of P and of Q after each step
   int grown[kMaxSteps + 1];            // X before each phase is at most 2^grown times X0
 };
-
-typedef __attribute__((address_space(3))) f16x8 lds_f16x8;
-typedef __attribute__((address_space(3))) f16x4 lds_f16x4;
-typedef __attribute__((address_space(3))) _Float16 lds_f16;
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-typedef __attribute__((address_space(3))) float lds_f32;
-template <typename P>
-__device__ __forceinline__ P* lds_ptr(unsigned at) {
-  return reinterpret_cast<P*>(static_cast<uintptr_t>(at));
-}
 
 // LDS rows of pairs (32 hi, 32 lo, ...), pitch a multiple of 256 B; 16-B chunk c of row r at c ^ sm_swz(r):
 // 16 rows of one chunk lie on distinct banks, and so do 64 B of 4 consecutive rows (a transposed read).
@@ -1322,15 +1342,21 @@ long long ns_tiles(const NsGroup& g, const NsJobs& js, int T) {
   return nt * ceil_div(g.np, T);
 }
 
-template <int T, int MODE, int OUT>
+template <int T, int MODE, int OUT, int G = 1>
 int ns_launch_tile(NsGroups& gs, const NsJobs& js, hipStream_t st) {
   const long long blocks = ns_grid(gs, [&](const NsGroup& g) { return ns_tiles<MODE>(g, js, T); });
   if (blocks == 0) return PROTOSEG_OK;
   if (int e = ns_blocks_ok(blocks)) return e;
-  constexpr size_t lds = static_cast<size_t>(ring_of(T)) * stage_bytes(T);
-  if (int e = ensure_lds<ns_product_kernel<T, MODE, OUT>, lds>()) return e;
+  if constexpr (MODE == kSym && G == 1) {
+    long long stages = 0;
+    for (int k = 0; k < gs.n; ++k)
+      stages = std::max<long long>(stages, js.j[0].l <= kX1 ? gs.g[k].np / 32 / (js.partial ? gs.g[k].split : 1) : gs.g[k].mp / 32);
+    if (blocks <= kHalvesTiles && stages >= kHalvesStages) return ns_launch_tile<T, MODE, OUT, 2>(gs, js, st);
+  }
+  constexpr size_t lds = static_cast<size_t>(G) * ring_of(T) * stage_bytes(T);
+  if (int e = ensure_lds<ns_product_kernel<T, MODE, OUT, G>, lds>()) return e;
   KernelTimer t("ns_product_kernel", st);
-  hipLaunchKernelGGL((ns_product_kernel<T, MODE, OUT>), dim3(static_cast<unsigned>(blocks)), dim3(256), lds, st, gs, js);
+  hipLaunchKernelGGL((ns_product_kernel<T, MODE, OUT, G>), dim3(static_cast<unsigned>(blocks)), dim3(256 * G), lds, st, gs, js);
   return check_launch("ns_product_kernel");
 }
 int ns_launch_thin(NsGroups& gs, const NsJobs& js, hipStream_t st) {

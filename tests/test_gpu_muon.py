@@ -98,6 +98,7 @@ def check_batch(out, g):
     (1, 64, 18432), (1, 20001, 70),  # the same with a split contraction
     (30, 130, 200),     # 64 x 64 tiles
     (12, 200, 2100), (12, 2100, 200),  # with a split contraction
+    (100, 64, 500), (90, 64, 570), (90, 570, 60), (5, 700, 800),  # two halves of a contraction beside each other
     (100, 257, 130), (100, 130, 257),  # 128 x 128 tiles of Q X
 ], ids=str)
 def test_every_kernel_path(device, shape, dtype):
