@@ -65,7 +65,19 @@ struct GnMap {  // element (b, pixel, c) at p[b * sb + pixel * sp + c]
 struct GnShape {
   int B, HW, C, G, cpg;
   int ppc, nchunk;  // pixels per chunk, chunks per sample
+  bool stream;      // NT of put_map, where vectors are 16 B
 };
+
+// A result beyond the L2s (8 x 4 MiB) is stored past the caches: kept there it would push out the map that the
+// second pass reads again (1 x 2048 x 129 x 257 bf16, three maps in turn: 80.8 us for 91.8, and 125 for 135 with
+// a reader behind it). A smaller one is left to the operation that reads it (3 x 150 x 33 x 47 f16 with a
+// reader: 24.7 us for 26.0).
+constexpr long long kGnStream = 32 << 20;
+template <bool NT, typename V>
+__device__ __forceinline__ void put_map(V* p, const V& v) {
+  if constexpr (NT) __builtin_nontemporal_store(v, p);
+  else *p = v;
+}
 
 // 1 / (1 + exp(-z)) by v_exp_f32 and v_rcp_f32 (1 ulp each; the exponent's argument is rounded
 // once, so the relative error is |z| 2^-24 + 2^-22): exact division and exp would make the 16-bit
@@ -288,7 +300,7 @@ __device__ __forceinline__ void load_coef(GnCoef<V, S>& k, const float4* cg, con
 // than a few thousand pairs read from L2 by each workgroup, many more than that do not.
 // 1 x 2048 x 129 x 257 bf16: 44.6 us, 6.1 TB/s read and written (56.7 without the next rows' loads in
 // flight while these are computed); 2 x 256 x 65 x 65 bf16: 9.3 us.
-template <typename T, int V, int S, int ACT>
+template <typename T, int V, int S, int ACT, bool NT>
 __global__ __launch_bounds__(kGnThreads) void gn_apply_kernel(GnMap x, GnShape s, GnParts pt, const double2* __restrict__ part,
                                                               double eps, double2* __restrict__ stat,
                                                               const float* __restrict__ w, const float* __restrict__ beta,
@@ -330,7 +342,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_apply_kernel(GnMap x, GnShape s
     unpack<T, V>(rx, v);
 #pragma unroll
     for (int i = 0; i < V; ++i) v[i] = act_of<ACT>(fmaf((v[i] - k.mh[i / S]) - k.ml[i / S], k.a[i], k.beta[i]));
-    *reinterpret_cast<vec*>(dst + static_cast<long long>(pp) * s.C) = pack<T, V>(v);
+    put_map<NT>(reinterpret_cast<vec*>(dst + static_cast<long long>(pp) * s.C), pack<T, V>(v));
   };
   while (p < p1) {
     vec n[kU];
@@ -474,7 +486,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_sums_kernel(GnMap x, GnMap 
 // samples (g_w, g_beta), 16 channels x 16 lanes each, so that their chain of loads runs beside the
 // map's. Either part may be absent. gpart / gsum: the groups' partials, or joined (gn_join_kernel).
 // 32 x 64 x 65 x 65 f32: 18.1 us, 5.7 TB/s.
-template <typename T, int V, int S, int ACT>
+template <typename T, int V, int S, int ACT, bool NT>
 __global__ __launch_bounds__(kGnThreads) void gn_bwd_apply_kernel(GnMap x, GnMap gy, GnShape s, GnParts pt, int nsum,
                                                                   const double2* __restrict__ stat,
                                                                   const float* __restrict__ w, const float* __restrict__ beta,
@@ -564,7 +576,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_apply_kernel(GnMap x, GnMap
       const float gz = grad_z<ACT>(g[i], v[i], d, k.a[i], k.beta[i], stat, w, b, c0 + i, s);
       v[i] = fmaf(k.a[i], gz, -fmaf(d, kk[i / S].y, kk[i / S].x));
     }
-    *reinterpret_cast<vec*>(dst + static_cast<long long>(pp) * s.C) = pack<T, V>(v);
+    put_map<NT>(reinterpret_cast<vec*>(dst + static_cast<long long>(pp) * s.C), pack<T, V>(v));
   };
   while (p < p1) {
     vec nx[kU], ng[kU];
@@ -658,7 +670,7 @@ int gn_shape(GnShape& s, int dtype, int B, int HW, int C, int G, double eps, int
   if (act < kGnIdentity || act > kGnSilu) return fail(PROTOSEG_ERR_INVALID, "group norm activation %d (0..3)", act);
   if (C > (1 << 20) || B > 65535 || HW > (1 << 30))
     return fail(PROTOSEG_ERR_UNSUPPORTED, "group norm B %d, HW %d, C %d (at most 65535, 2^30, 2^20)", B, HW, C);
-  s = GnShape{B, HW, C, G, C / G, 0, 0};
+  s = GnShape{B, HW, C, G, C / G, 0, 0, static_cast<long long>(B) * HW * C * (dtype == PROTOSEG_F32 ? 4 : 2) > kGnStream};
   if (B > 0 && HW > 0) gn_chunks(s);
   return PROTOSEG_OK;
 }
@@ -734,8 +746,13 @@ extern "C" int protoseg_group_norm_fwd(const void* x, int x_dtype, int B, int HW
                          dim3(kGnThreads), 0, st, part, s, pt, eps, stat);
     return gn_act(act_kind, [&](auto act) -> int {
       KernelTimer t("gn_apply_kernel", st);
-      hipLaunchKernelGGL((gn_apply_kernel<T, kV, kS, decltype(act)::value>), grid, dim3(kGnThreads), 0, st, m, s, pt,
-                         inside ? part : nullptr, eps, stat, weight, bias, static_cast<T*>(y));
+      auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(kGnThreads), 0, st, m, s, pt, inside ? part : nullptr, eps, stat, weight, bias,
+                           static_cast<T*>(y));
+      };
+      constexpr bool kMay = kV * sizeof(T) == 16;
+      if (kMay && s.stream) go(gn_apply_kernel<T, kV, kS, decltype(act)::value, kMay>);
+      else go(gn_apply_kernel<T, kV, kS, decltype(act)::value, false>);
       return check_launch("group norm forward");
     });
   });
@@ -784,9 +801,14 @@ extern "C" int protoseg_group_norm_bwd(const void* x, const void* g_y, int x_dty
                            dim3(kGnThreads), 0, st, gpart, s, pt, 0.0, gsum);
       const unsigned nsum = g_weight || g_bias ? static_cast<unsigned>(ceil_div(C, 16)) : 0u;
       KernelTimer t("gn_bwd_apply_kernel", st);
-      hipLaunchKernelGGL((gn_bwd_apply_kernel<T, kV, kS, kAct>), dim3((g_x ? nmap : 0u) + nsum, static_cast<unsigned>(pt.gy)),
-                         dim3(kGnThreads), 0, st, m, mg, s, pt, static_cast<int>(nsum), stat, weight, bias, part, gpart,
-                         inside ? nullptr : gsum, static_cast<T*>(g_x), g_weight, g_bias);
+      auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((g_x ? nmap : 0u) + nsum, static_cast<unsigned>(pt.gy)), dim3(kGnThreads), 0, st, m, mg,
+                           s, pt, static_cast<int>(nsum), stat, weight, bias, part, gpart, inside ? nullptr : gsum,
+                           static_cast<T*>(g_x), g_weight, g_bias);
+      };
+      constexpr bool kMay = kV * sizeof(T) == 16;
+      if (kMay && s.stream) go(gn_bwd_apply_kernel<T, kV, kS, kAct, kMay>);
+      else go(gn_bwd_apply_kernel<T, kV, kS, kAct, false>);
       return check_launch("group norm backward");
     });
   });
