@@ -22,8 +22,8 @@ namespace protoseg {
 namespace {
 
 constexpr int kGnThreads = 256;
-constexpr long long kGnTarget = 512, kGnLeast = 4096, kGnEnough = 16384;  // gn_chunks
-constexpr long long kGnJoinInside = 4096;                               // gn_apply_kernel
+constexpr long long kGnTarget = 512, kGnLeast = 4096, kGnEnough = 16384, kGnMost = 1 << 18;  // gn_chunks
+constexpr long long kGnJoinInside = 4096;  // gn_apply_kernel
 
 enum GnAct { kGnIdentity = 0, kGnRelu = 1, kGnSigmoid = 2, kGnSilu = 3 };
 
@@ -382,8 +382,8 @@ __device__ __forceinline__ float grad_z(float gy, float x, float d, float a, flo
 
 // Partial sums of one chunk, S1 = sum gz and S2 = sum gz xh: per channel (part, f32 rows [2][C] of
 // each workgroup), and weighted by w over each group (gpart). f32 inside a chunk, where a thread adds up
-// ppc / R values of mixed sign (8 to 67 in this library's maps; more where a large batch leaves one chunk a
-// sample); the chunks are joined in f64. 32 x 64 x 65 x 65 f32: 14.7 us, 4.7 TB/s.
+// ppc / R values of mixed sign (8 to 67 in this library's maps, about 1024 / V at most); the chunks are joined
+// in f64. 32 x 64 x 65 x 65 f32: 14.7 us, 4.7 TB/s.
 template <typename T, int V, int S, int ACT>
 __global__ __launch_bounds__(kGnThreads) void gn_bwd_sums_kernel(GnMap x, GnMap gy, GnShape s, GnParts pt,
                                                                  const double2* __restrict__ stat,
@@ -610,11 +610,13 @@ __global__ void gn_zero_kernel(float* a, float* b, int n) {
 // 257 x 257 bf16 50.2 us for 45.5), none below 4096 elements (3 x 150 x 33 x 47 f16: 20.4 us, with 16384
 // 29.7). Where every workgroup of the second pass would join more than 2048 pairs of a sample, shorter chunks cost
 // as much as they save: 16384 elements then (2 x 256 x 65 x 65 bf16: 34.2 us, with 4096 37.1).
+// None above 2^18 elements, which bounds the chains of gn_bwd_sums_kernel.
 void gn_chunks(GnShape& s) {
   long long want = ceil_div(kGnTarget, s.B);
   const long long all = static_cast<long long>(s.HW) * s.C, inside = kGnJoinInside / 2 / s.G, enough = ceil_div(all, kGnEnough);
   if (want > ceil_div(all, kGnLeast)) want = ceil_div(all, kGnLeast);
   if (want > inside && want > enough) want = inside > enough ? inside : enough;
+  if (want < ceil_div(all, kGnMost)) want = ceil_div(all, kGnMost);
   if (want > s.HW) want = s.HW;
   if (want < 1) want = 1;
   s.ppc = static_cast<int>(ceil_div(s.HW, want));

@@ -131,6 +131,18 @@ def test_forward_and_backward(device, shape, dtype):
         close(got, ref, key)
 
 
+@pytest.mark.parametrize("shape,dtype,act", [((2, 64, 271, 263), torch.float32, "silu"), ((1, 512, 181, 189), torch.bfloat16, "relu"),
+                                             ((1, 516, 181, 189), torch.float16, "identity")], ids=str)
+def test_maps_beyond_the_caches(device, shape, dtype, act):
+    """Results of more than 32 MiB, in 16-B vectors and (516 halves) in 4-B ones."""
+    x, w, b, gy = make(device, *shape, dtype, 19)
+    assert x.numel() * x.element_size() > 32 << 20
+    got = run(x, 4, w, b, 1e-5, act, gy)
+    ref = reference(x, 4, w, b, 1e-5, act, gy)
+    for v, key in zip(got, ("y", "gx", "gw", "gb")):
+        close(v, ref, key)
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("layout", ["cl", "nchw", "slice", "odd"])
 def test_layouts_and_activations(device, layout, act):
