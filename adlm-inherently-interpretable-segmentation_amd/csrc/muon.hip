@@ -397,9 +397,11 @@ __device__ __forceinline__ void stage_wait(int later) {
 // stages of 32 k, ring_of - 1 ahead of the products, with one barrier a stage. In the step over a ResNet-101's
 // convolutions (109 matrices, 47e6 elements) the Gram product takes 109 us, Q X 142 us, Q X with the parameters'
 // update 177 us, a product of squares 30 us: 524, 677, 545 and 410 TFLOP/s of f16, where a large library product
-// reaches 1100. LDS bounds a 64 x 64 tile: a stage is 192 cycles of MFMA on each SIMD, and 32 KiB read and 16 KiB
-// written at 128 B a cycle are 384. At 128 x 128 they are even (768 and 768), but the symmetric products would
-// compute a fifth more and leave half the chip's places empty at the end (measured slower).
+// reaches 1100. No single unit is full in the Gram product: a stage of a 64 x 64 tile is 192 cycles of MFMA on each
+// SIMD (23 us in all) and 384 of LDS (32 KiB read and 16 KiB written at 128 B a cycle: 45 us), and L2 serves 10 TB/s;
+// without MFMAs 84 % of its time stayed, without the loads 67 %: it waits for loads, with three workgroups a CU. At
+// 128 x 128 LDS is read half as often, but the symmetric products would compute a fifth more and leave half the
+// chip's places empty at the end (measured slower).
 // G = 2: a second set of 4 waves takes the second half of the stages and hands its sums over at the end.
 template <int T, int MODE, int OUT, int G = 1>
 __global__ __launch_bounds__(256 * G, 160 * 1024 / (G * ring_of(T) * stage_bytes(T))) void ns_product_kernel(NsGroups gs, NsJobs js) {

@@ -298,7 +298,7 @@ __device__ __forceinline__ void load_coef(GnCoef<V, S>& k, const float4* cg, con
 // y = act(z). part: the statistics' partials, joined here by every workgroup (the first chunk's
 // leave them in `stat`), or null where gn_join_kernel has joined them: a launch less costs more
 // than a few thousand pairs read from L2 by each workgroup, many more than that do not.
-// 1 x 2048 x 129 x 257 bf16: 44.6 us, 6.1 TB/s read and written (56.7 without the next rows' loads in
+// 1 x 2048 x 129 x 257 bf16: 44.2 us, 6.1 TB/s read and written (56.7 without the next rows' loads in
 // flight while these are computed); 2 x 256 x 65 x 65 bf16: 9.3 us.
 template <typename T, int V, int S, int ACT, bool NT>
 __global__ __launch_bounds__(kGnThreads) void gn_apply_kernel(GnMap x, GnShape s, GnParts pt, const double2* __restrict__ part,
