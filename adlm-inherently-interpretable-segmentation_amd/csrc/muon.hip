@@ -8,9 +8,9 @@
 //   A = X X^T;   per step  P = a I + b A + c A A,  Q <- P Q,  A <- P A P;   X <- Q X.
 // For an m x n matrix that is 3 m^2 n + O(m^3) multiply-adds a phase against 4 m^2 n a step. A's rounding
 // (2^-22 of its norm) can leave a zero eigenvalue slightly negative, and every step multiplies it by a^2:
-// a phase is cut where that could reach 2^-13 (3 steps at a = 3.4445), and the next one starts from a new
-// X X^T, which has no negative eigenvalues. The default five steps run as 3 + 2, or in shorter phases where
-// the result is to be exact to f32 (ns_exact_longest).
+// a phase is cut after two steps at most (one where the result would lose by it, ns_longest), or where that
+// could reach 2^-13, and the next one starts from a new X X^T, which has no negative eigenvalues. The default
+// five steps run as 2 + 2 + 1 or one by one.
 //
 // Products run on v_mfma_f32_32x32x16_f16 with every operand held as a pair of f16 values, hi + lo of the
 // value times a power of two (22 bits, no overflow: singular values are bounded by the scalar map, checked
@@ -81,6 +81,7 @@ struct NsTarget {
 // of their own it was two half lines and twice the requests to L2, at the same time.)
 struct NsGroup {
   int m, n, mp, np, count, tall;
+  int kind;          // which of a call's two plans its steps follow (ns_kind)
   int split;         // workgroups along the Gram contraction
   int chunks, target;  // chunks of the sums of squares; index of the first matrix's NsTarget and sums
   long long x, sq, part;
@@ -360,11 +361,16 @@ __device__ __forceinline__ int x_shift(const NsTarget& t, int grown) { return ma
 __device__ __forceinline__ const NsTarget& target_of(const NsGroups& gs, const NsGroup& g, int mat) {
   return reinterpret_cast<const NsTarget*>(gs.ws + gs.targets)[g.target + mat];
 }
-struct NsJobs {
+struct NsPart {    // what a group does in a launch (n = 0: nothing)
   NsJob j[2];
   int n;
-  float a, b, c;   // poly
   int partial;     // groups with split > 1 leave f32 partials (ns_join_kernel makes the result)
+};
+// Per group, not per kind: read with the group itself, where a second level of loads from the arguments costs every
+// launch 1.3 us (22 matrices of 256 x 1024: 210 us for 187).
+struct NsJobs {
+  NsPart of[kMaxGroups];
+  float a, b, c;   // poly
 };
 
 enum NsMode { kSym = 0, kApply = 1, kWide = 2, kTall = 3 };
@@ -418,8 +424,9 @@ __global__ __launch_bounds__(256 * G, 160 * 1024 / (G * ring_of(T) * stage_bytes
   const NsGroup& g = gs.g[gi];
   const int nt = (g.mp + T - 1) / T, nc = KX ? (g.np + T - 1) / T : nt;
   const int tiles = KX ? nt * nc : nt * (nt + 1) / 2;
-  const int splits = MODE == kSym && js.partial ? g.split : 1;
-  const int per = tiles * splits * (MODE == kSym ? js.n : 1);
+  const NsPart& jp = js.of[gi];
+  const int splits = MODE == kSym && jp.partial ? g.split : 1;
+  const int per = tiles * splits * (MODE == kSym ? jp.n : 1);
   int local = xcd_local(static_cast<int>(blockIdx.x) - gs.first[gi], per * g.count);
   if (local < 0) return;
   const int mat = local / per;
@@ -435,7 +442,7 @@ __global__ __launch_bounds__(256 * G, 160 * 1024 / (G * ring_of(T) * stage_bytes
     while (tile >= nt - ti) tile -= nt - ti, ++ti;
     tc = ti + tile;
   }
-  NsJob job = js.j[jb];
+  NsJob job = jp.j[jb];
   if (MODE == kSym && job.l <= kX1) job.inv = ldexpf(job.inv, -2 * x_shift(target_of(gs, g, mat), job.grown));
   const int K = MODE == kSym && job.l <= kX1 ? g.np : g.mp;
   const int i0 = ti * T, c0 = tc * T;
@@ -566,7 +573,7 @@ __global__ __launch_bounds__(256 * G, 160 * 1024 / (G * ring_of(T) * stage_bytes
       const int ib = i0 + wi + 32 * a, cb = c0 + wc + 32 * b;  // the block's first row and column
       if (ib >= g.mp || cb >= (KX ? g.np : g.mp)) continue;
       if constexpr (MODE == kSym) {
-        if (js.partial && g.split > 1) {
+        if (jp.partial && g.split > 1) {
           float* dst = reinterpret_cast<float*>(gs.ws + g.part) +
                        (static_cast<long long>(mat) * g.split + z) * g.mp * g.mp + static_cast<long long>(ib) * g.mp + cb + j;
 #pragma unroll
@@ -657,7 +664,8 @@ __global__ __launch_bounds__(256, 1) void ns_thin_kernel(NsGroups gs, NsJobs js)
   const int lane = threadIdx.x & 63, wave = bf16l::wave_id(), j = lane & 31, h = lane >> 5;
   const int gi = place_of(gs.first, blockIdx.x);
   const NsGroup& g = gs.g[gi];
-  const int nt = g.mp / 32, tiles = nt * (nt + 1) / 2, splits = js.partial ? g.split : 1, per = tiles * splits * js.n;
+  const NsPart& jp = js.of[gi];
+  const int nt = g.mp / 32, tiles = nt * (nt + 1) / 2, splits = jp.partial ? g.split : 1, per = tiles * splits * jp.n;
   int local = xcd_local(static_cast<int>(blockIdx.x) - gs.first[gi], per * g.count);
   if (local < 0) return;
   const int mat = local / per;
@@ -668,7 +676,7 @@ __global__ __launch_bounds__(256, 1) void ns_thin_kernel(NsGroups gs, NsJobs js)
   int tile = local - z * tiles, ti = 0;
   while (tile >= nt - ti) tile -= nt - ti, ++ti;
   const int i0 = 32 * ti, c0 = 32 * (ti + tile);
-  NsJob job = js.j[jb];
+  NsJob job = jp.j[jb];
   if (job.l <= kX1) job.inv = ldexpf(job.inv, -2 * x_shift(target_of(gs, g, mat), job.grown));
   const int K = job.l <= kX1 ? g.np : g.mp, nst_all = K / 32;
   const int st0 = nst_all * z / splits, nst = nst_all * (z + 1) / splits - st0;
@@ -727,7 +735,7 @@ __global__ __launch_bounds__(256, 1) void ns_thin_kernel(NsGroups gs, NsJobs js)
     for (int w = 0; w < 4; ++w) v[e] += reinterpret_cast<const float*>(sm + w * kThinRing * kThinStage)[64 * (4 * wave + e) + lane];
   }
   const int row = i0 + 8 * wave + 4 * h, col = c0 + j;
-  if (js.partial && g.split > 1) {
+  if (jp.partial && g.split > 1) {
     float* dst = reinterpret_cast<float*>(gs.ws + g.part) +
                  (static_cast<long long>(mat) * g.split + z) * g.mp * g.mp + static_cast<long long>(row) * g.mp + col;
 #pragma unroll
@@ -762,7 +770,7 @@ __global__ __launch_bounds__(256, 1) void ns_thin_kernel(NsGroups gs, NsJobs js)
 // The partials of a split Gram product joined in a fixed order (8.0 us in the 109 matrices' step, bound by reading
 // them): a workgroup takes one 32 x 32 block on or
 // above the diagonal, each wave every fourth split, and stores it with its mirror image.
-__global__ __launch_bounds__(256) void ns_join_kernel(NsGroups gs, float inv, int grown) {
+__global__ __launch_bounds__(256) void ns_join_kernel(NsGroups gs, NsJobs js) {
   __shared__ float red[3][16][64];
   const int gi = place_of(gs.first, blockIdx.x);
   const NsGroup& g = gs.g[gi];
@@ -790,7 +798,8 @@ __global__ __launch_bounds__(256) void ns_join_kernel(NsGroups gs, float inv, in
   }
   __syncthreads();
   if (wave) return;
-  inv = ldexpf(inv, -2 * x_shift(target_of(gs, g, mat), grown));
+  const NsJob& job = js.of[gi].j[0];
+  const float inv = ldexpf(job.inv * job.so, -2 * x_shift(target_of(gs, g, mat), job.grown));
   _Float16* hi = pairs_of(gs, g, kA, mat);
   Pair p[16];
 #pragma unroll
@@ -1181,15 +1190,27 @@ float scale_for(double most) {  // the largest power of two up to kScale that ke
   return s;
 }
 
-// The longest phase for a result of 22 bits or more: A's rounding, amplified along a phase, falls on the small
-// singular directions, and near-square matrices have them. Error of five steps over that of f32 products,
-// noise matrices: phases of 3 + 2 1.5 (64 x 128), 1.7 (64 x 64); 2 + 2 + 1 0.6 and 1.4; 1 + 1 + 1 + 1 + 1
-// 0.5 and 0.6. Single steps cost no more where n < 1.5 m. A 16-bit result, and an update that is scaled
-// into the parameters, do not show the difference: 3 + 2 there (two products of m^2 n less).
-constexpr int kLongest = 3;
-int ns_exact_longest(int rows, int cols) {
+// The longest phase. A's rounding, amplified along a phase, falls on the small singular directions, and narrow or
+// near-square matrices have them, while the sums of a wide product hide it. Error of five steps over that of
+// the formula in f32 products, noise matrices in f32, by phases:
+//             16x64  32x128  64x64  64x256  96x96  96x192  256x1024
+//   3 + 2      1.31    1.19   2.01    1.18   1.68    1.74      1.19
+//   2 + 2 + 1  2.05    2.25   1.52    1.50   1.35    0.77      0.54
+//   single     1.08    1.19   0.64    0.92   0.53    0.46      0.53
+// A 16-bit result shows it in its last bits (64 x 128 bf16: with 3 + 2 2.8e-3 of the elements rounded to the other
+// side, 1.0e-3 by the formula), an update in its parameters (the step over a ResNet-101's convolutions: 7.1e-8 of
+// them with 3 + 2, 6.4e-8 by the formula). So every type takes single steps below kNarrow rows and where n < 1.5 m,
+// and 2 + 2 + 1 elsewhere. Longer phases save products of m^2 n only: 22 x 256 x 1024 bf16 takes 172 us with 3 + 2,
+// 187 with 2 + 2 + 1, 201 with single steps.
+constexpr int kNarrow = 96;
+constexpr int kLongest[2] = {1, 2};  // of each kind
+// A call that has both kinds takes single steps for all, unless m^2 n of the wider ones (kind 1) is beyond this: the
+// kinds' launches go together only in part. 2 of 64 x 576 and 12, 24, 48 of 256 x 1024 (8e8, 1.6e9, 3.2e9):
+// 182, 225, 374 us with single steps for 202, 229, 369; 109 convolutions (1.6e10): 1544 for 1357.
+constexpr double kMixedLeast = 1.5e9;
+int ns_kind(int rows, int cols) {
   const long long m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
-  return 2 * n < 3 * m ? 1 : 2;
+  return m < kNarrow || 2 * n < 3 * m ? 0 : 1;
 }
 
 // Phases, and scales that keep every f16 in range: the singular values of X0 are at most 1 (the Frobenius
@@ -1260,6 +1281,7 @@ size_t ns_layout(NsGroups& gs, const std::vector<NsMatrix>& mats, std::vector<in
       g.n = g.tall ? mats[i].rows : mats[i].cols;
       g.mp = pad_of(g.m);
       g.np = pad_of(g.n);
+      g.kind = ns_kind(g.m, g.n);
     }
     if (which) {
       which->push_back(k);
@@ -1321,14 +1343,14 @@ int ns_check(int rows, int cols) {
   return PROTOSEG_OK;
 }
 
-// first[] of every group for a launch that gives each of its matrices per(g) workgroups; the grid.
+// first[] of every group for a launch that gives each matrix of group k per(k) workgroups; the grid.
 template <typename F>
 long long ns_grid(NsGroups& gs, F per) {
   long long blocks = 0;
   for (int k = gs.n; k < kMaxGroups; ++k) gs.first[k] = 0x7fffffff;
   for (int k = 0; k < gs.n; ++k) {
     gs.first[k] = static_cast<int>(blocks < (1LL << 30) ? blocks : (1LL << 30));
-    blocks += (per(gs.g[k]) * gs.g[k].count + 7) / 8 * 8;
+    blocks += (per(k) * gs.g[k].count + 7) / 8 * 8;
   }
   return blocks;
 }
@@ -1337,22 +1359,25 @@ int ns_blocks_ok(long long blocks) {
 }
 
 template <int MODE>
-long long ns_tiles(const NsGroup& g, const NsJobs& js, int T) {
+long long ns_tiles(const NsGroup& g, const NsPart& jp, int T) {
   const long long nt = ceil_div(g.mp, T);
-  if (MODE == kSym) return nt * (nt + 1) / 2 * js.n * (js.partial ? g.split : 1);
-  if ((MODE == kWide && g.tall) || (MODE == kTall && !g.tall)) return 0;
+  if (MODE == kSym) return nt * (nt + 1) / 2 * jp.n * (jp.partial ? g.split : 1);
+  if (!jp.n || (MODE == kWide && g.tall) || (MODE == kTall && !g.tall)) return 0;
   return nt * ceil_div(g.np, T);
 }
 
 template <int T, int MODE, int OUT, int G = 1>
 int ns_launch_tile(NsGroups& gs, const NsJobs& js, hipStream_t st) {
-  const long long blocks = ns_grid(gs, [&](const NsGroup& g) { return ns_tiles<MODE>(g, js, T); });
+  const long long blocks = ns_grid(gs, [&](int k) { return ns_tiles<MODE>(gs.g[k], js.of[k], T); });
   if (blocks == 0) return PROTOSEG_OK;
   if (int e = ns_blocks_ok(blocks)) return e;
   if constexpr (MODE == kSym && G == 1) {
     long long stages = 0;
-    for (int k = 0; k < gs.n; ++k)
-      stages = std::max<long long>(stages, js.j[0].l <= kX1 ? gs.g[k].np / 32 / (js.partial ? gs.g[k].split : 1) : gs.g[k].mp / 32);
+    for (int k = 0; k < gs.n; ++k) {
+      const NsGroup& g = gs.g[k];
+      const NsPart& jp = js.of[k];
+      if (jp.n) stages = std::max<long long>(stages, jp.j[0].l <= kX1 ? g.np / 32 / (jp.partial ? g.split : 1) : g.mp / 32);
+    }
     if (blocks <= kHalvesTiles && stages >= kHalvesStages) return ns_launch_tile<T, MODE, OUT, 2>(gs, js, st);
   }
   constexpr size_t lds = static_cast<size_t>(G) * ring_of(T) * stage_bytes(T);
@@ -1362,7 +1387,7 @@ int ns_launch_tile(NsGroups& gs, const NsJobs& js, hipStream_t st) {
   return check_launch("ns_product_kernel");
 }
 int ns_launch_thin(NsGroups& gs, const NsJobs& js, hipStream_t st) {
-  const long long blocks = ns_grid(gs, [&](const NsGroup& g) { return ns_tiles<kSym>(g, js, 32); });
+  const long long blocks = ns_grid(gs, [&](int k) { return ns_tiles<kSym>(gs.g[k], js.of[k], 32); });
   constexpr size_t lds = 4 * kThinRing * kThinStage;
   if (int e = ensure_lds<ns_thin_kernel, lds>()) return e;
   KernelTimer t("ns_thin_kernel", st);
@@ -1375,74 +1400,107 @@ int ns_launch(NsGroups gs, const NsJobs& js, hipStream_t st) {
     return gs.thin ? ns_launch_thin(gs, js, st) : ns_launch_tile<64, MODE, OUT>(gs, js, st);
   } else {
     long long big = 0;
-    for (int k = 0; k < gs.n; ++k) big += ns_tiles<MODE>(gs.g[k], js, 128) * gs.g[k].count;
+    for (int k = 0; k < gs.n; ++k) big += ns_tiles<MODE>(gs.g[k], js.of[k], 128) * gs.g[k].count;
     return big >= kApplyTiles ? ns_launch_tile<128, MODE, OUT>(gs, js, st) : ns_launch_tile<64, MODE, OUT>(gs, js, st);
   }
 }
 
-// All products of a prepared X0, ending in the targets.
-template <int OUT>
-int ns_products(const NsGroups& gs, const NsPlan& pl, hipStream_t st) {
+// The launches of a plan, in order.
+enum NsLaunch { kSymmetric = 0, kNextX = 1, kResult = 2 };
+struct NsOp {
+  NsLaunch launch;
+  NsPart part;
+};
+std::vector<NsOp> ns_program(const NsPlan& pl, bool split) {
+  std::vector<NsOp> ops;
   int x = kX0, step = 0;
-  auto sym = [&](std::initializer_list<NsJob> jobs, int partial = 0) {
-    NsJobs js{};
-    for (const NsJob& j : jobs) js.j[js.n++] = j;
-    js.a = pl.a, js.b = pl.b, js.c = pl.c, js.partial = partial;
-    return ns_launch<kSym, kOutF32>(gs, js, st);
+  auto add = [&](NsLaunch launch, std::initializer_list<NsJob> jobs, int partial = 0) {
+    NsOp op{launch, NsPart{}};
+    for (const NsJob& j : jobs) op.part.j[op.part.n++] = j;
+    op.part.partial = partial;
+    ops.push_back(op);
   };
-  bool split = false;
-  for (int k = 0; k < gs.n; ++k) split = split || gs.g[k].split > 1;
   for (int p = 0; p < pl.nphase; ++p) {
-    if (int e = sym({NsJob{x, x, kA, 0, 1.f / (kScale * kScale), kScale, pl.grown[p]}}, split)) return e;
-    if (split) {
-      NsGroups js = gs;
-      const long long blocks = ns_grid(js, [](const NsGroup& g) -> long long {
-        const long long nb = g.mp / 32;
-        return g.split > 1 ? nb * (nb + 1) / 2 : 0;
-      });
-      hipLaunchKernelGGL(ns_join_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, js, 1.f / kScale, pl.grown[p]);
-      if (int e = check_launch("ns_join_kernel")) return e;
-    }
+    add(kSymmetric, {NsJob{x, x, kA, 0, 1.f / (kScale * kScale), kScale, pl.grown[p]}}, split);
     int q = kQ0;
     float sq = 0.f;
     for (int k = 0; k < pl.phases[p]; ++k, ++step) {
       const float sp = pl.sp[step];
       const int pb = k == 0 ? kQ0 : kP;  // the first P is Q
-      if (int e = sym({NsJob{kA, kA, pb, 1, 1.f / (kScale * kScale), sp}})) return e;
+      add(kSymmetric, {NsJob{kA, kA, pb, 1, 1.f / (kScale * kScale), sp}});
       const bool more = k + 1 < pl.phases[p];
       const NsJob mul{pb, kA, kT, 0, 1.f / (sp * kScale), kScale};
       if (k == 0) {
         sq = sp;
-        if (more)
-          if (int e = sym({mul})) return e;
+        if (more) add(kSymmetric, {mul});
       } else {
         const int qn = q == kQ0 ? kQ1 : kQ0;
         const NsJob acc{pb, q, qn, 0, 1.f / (sp * sq), pl.sq[step]};
-        if (int e = more ? sym({mul, acc}) : sym({acc})) return e;
+        if (more) add(kSymmetric, {mul, acc});
+        else add(kSymmetric, {acc});
         q = qn;
         sq = pl.sq[step];
       }
-      if (more)
-        if (int e = sym({NsJob{kT, pb, kA, 0, 1.f / (sp * kScale), kScale}})) return e;
+      if (more) add(kSymmetric, {NsJob{kT, pb, kA, 0, 1.f / (sp * kScale), kScale}});
     }
-    NsJobs js{};
-    js.n = 1;
     if (p + 1 < pl.nphase) {
       const int xn = x == kX0 ? kX1 : kX0;
-      js.j[0] = NsJob{q, x, xn, 0, 1.f / (sq * kScale), kScale, pl.grown[p], pl.grown[p + 1]};
-      if (int e = ns_launch<kApply, kOutF32>(gs, js, st)) return e;
+      add(kNextX, {NsJob{q, x, xn, 0, 1.f / (sq * kScale), kScale, pl.grown[p], pl.grown[p + 1]}});
       x = xn;
     } else {
-      js.j[0] = NsJob{q, x, x, 0, 1.f / (sq * kScale), 1.f, pl.grown[p]};
+      add(kResult, {NsJob{q, x, x, 0, 1.f / (sq * kScale), 1.f, pl.grown[p]}});
+    }
+  }
+  return ops;
+}
+
+// All products of a prepared X0, ending in the targets. pl[kind]: the plan of each kind that is there. Two kinds share
+// launches: a kind whose X is due waits for no other, and symmetric products of both go together (five steps of
+// 1 + 1 + 1 + 1 + 1 beside 2 + 2 + 1: 21 launches, 17 and 15 alone).
+template <int OUT>
+int ns_products(const NsGroups& gs, const NsPlan (&pl)[2], hipStream_t st) {
+  bool split = false, there[2] = {false, false};
+  for (int k = 0; k < gs.n; ++k) split = split || gs.g[k].split > 1, there[gs.g[k].kind] = true;
+  std::vector<NsOp> ops[2];
+  for (int c = 0; c < 2; ++c)
+    if (there[c]) ops[c] = ns_program(pl[c], split);
+  size_t at[2] = {0, 0};
+  while (at[0] < ops[0].size() || at[1] < ops[1].size()) {
+    NsLaunch launch = kSymmetric;
+    for (int c = 0; c < 2; ++c)
+      if (at[c] < ops[c].size()) launch = std::max(launch, ops[c][at[c]].launch);
+    NsJobs js{};
+    for (int c = 0; c < 2; ++c) {
+      if (!there[c]) continue;
+      js.a = pl[c].a, js.b = pl[c].b, js.c = pl[c].c;
+      if (at[c] == ops[c].size() || ops[c][at[c]].launch != launch) continue;
+      for (int k = 0; k < gs.n; ++k)
+        if (gs.g[k].kind == c) js.of[k] = ops[c][at[c]].part;
+      ++at[c];
+    }
+    if (launch == kNextX) {
+      if (int e = ns_launch<kApply, kOutF32>(gs, js, st)) return e;
+    } else if (launch == kResult) {
       if (int e = ns_launch<kWide, OUT>(gs, js, st)) return e;
       if (int e = ns_launch<kTall, OUT>(gs, js, st)) return e;
+    } else {
+      if (int e = ns_launch<kSym, kOutF32>(gs, js, st)) return e;
+      NsGroups parts = gs;
+      const long long blocks = ns_grid(parts, [&](int k) -> long long {
+        const long long nb = gs.g[k].mp / 32;
+        return js.of[k].partial && gs.g[k].split > 1 ? nb * (nb + 1) / 2 : 0;
+      });
+      if (blocks) {
+        hipLaunchKernelGGL(ns_join_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, parts, js);
+        if (int e = check_launch("ns_join_kernel")) return e;
+      }
     }
   }
   return PROTOSEG_OK;
 }
 
 // Beside larger matrices a small one is nearly free in their launches; the kernel of its own is for calls
-// that have no others.
+// that have no others. All of these are of kind 0.
 bool ns_is_small(int rows, int cols) {
   const int m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
   return m <= kSmallM && pad_of(n) <= kSmallN;
@@ -1520,8 +1578,9 @@ extern "C" int protoseg_orthogonalize(const void* g, int dtype, int count, int r
   if (count < 0) return fail(PROTOSEG_ERR_INVALID, "orthogonalize: %d matrices", count);
   if (int e = ns_check(rows, cols)) return e;
   if (!(eps >= 0.f)) return fail(PROTOSEG_ERR_INVALID, "orthogonalize eps %g", eps);
-  NsPlan pl;
-  if (int e = ns_plan(pl, steps, a, b, c, dtype == PROTOSEG_F32 ? ns_exact_longest(rows, cols) : kLongest)) return e;
+  NsPlan pl[2];
+  const int kind = ns_kind(rows, cols);
+  if (int e = ns_plan(pl[kind], steps, a, b, c, kLongest[kind])) return e;
   if (count == 0 || rows == 0 || cols == 0) return PROTOSEG_OK;
   const long long size = static_cast<long long>(rows) * cols;
   if (!g || !out) return fail(PROTOSEG_ERR_INVALID, "orthogonalize: matrices and result must be non-null");
@@ -1535,7 +1594,7 @@ extern "C" int protoseg_orthogonalize(const void* g, int dtype, int count, int r
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const std::vector<NsItem> items{NsItem{g, static_cast<float*>(out), nullptr, stride, size, count, rows, cols, 0, 0, 0.f, 0.f}};
   auto go = [&](auto tag, auto kind) -> int {
-    if (is_small) return ns_small<decltype(tag), false>(items, pl, 0.f, 0, eps, st);
+    if (is_small) return ns_small<decltype(tag), false>(items, pl[0], 0.f, 0, eps, st);
     if (int e = ns_load<decltype(tag), false>(gs, items, 0.f, 0, eps, st)) return e;
     return ns_products<decltype(kind)::value>(gs, pl, st);
   };
@@ -1595,8 +1654,19 @@ extern "C" int protoseg_muon_step(int n_tensors, float* const* params, const flo
   if (!(momentum >= 0.f && momentum < 1.f) || !(eps >= 0.f) || !std::isfinite(lr) || !std::isfinite(weight_decay))
     return fail(PROTOSEG_ERR_INVALID, "muon: momentum %g in [0, 1), eps %g >= 0, lr %g, weight decay %g", momentum, eps, lr, weight_decay);
   if (scale_kind != 0 && scale_kind != 1) return fail(PROTOSEG_ERR_INVALID, "muon scale kind %d (0 or 1)", scale_kind);
-  NsPlan pl;
-  if (int e = ns_plan(pl, steps, a, b, c, kLongest)) return e;
+  NsPlan pl[2];
+  bool there[2] = {n_tensors == 0, false};
+  double wide = 0.0;  // m^2 n of the matrices of kind 1
+  for (int i = 0; i < n_tensors; ++i) {
+    const int k = ns_kind(rows[i], cols[i]);
+    there[k] = true;
+    if (k) wide += static_cast<double>(std::min(rows[i], cols[i])) * rows[i] * cols[i];
+  }
+  const bool single = there[0] && wide < kMixedLeast;
+  if (single) there[1] = false;
+  for (int k = 0; k < 2; ++k)
+    if (there[k])
+      if (int e = ns_plan(pl[k], steps, a, b, c, kLongest[k])) return e;
   std::vector<MuonRun> runs;
   if (int e = muon_runs(runs, n_tensors, rows, cols)) return e;
   size_t need = 0;
@@ -1630,6 +1700,7 @@ extern "C" int protoseg_muon_step(int n_tensors, float* const* params, const flo
     NsGroups gs;
     std::vector<int> which, index;
     ns_layout(gs, run.mats, &which, &index);
+    for (int k = 0; single && k < gs.n; ++k) gs.g[k].kind = 0;
     gs.ws = static_cast<unsigned char*>(workspace);
     items.clear();
     for (size_t k = 0; k < run.mats.size(); ++k) items.push_back(item(run.from[k], which[k], index[k]));
@@ -1639,7 +1710,7 @@ extern "C" int protoseg_muon_step(int n_tensors, float* const* params, const flo
   if (!runs.empty()) return PROTOSEG_OK;
   for (int i = 0; i < n_tensors; ++i)
     if (rows[i] && cols[i]) items.push_back(item(i, 0, 0));
-  return ns_small<float, true>(items, pl, momentum, nesterov ? 1 : 0, eps, st);
+  return ns_small<float, true>(items, pl[0], momentum, nesterov ? 1 : 0, eps, st);
 } catch (const std::exception& e) {
   return fail(PROTOSEG_ERR_INVALID, "muon: %s", e.what());
 }
