@@ -138,7 +138,7 @@ __device__ __forceinline__ T wave_part_sum(T v, int lanes) {  // over aligned ru
   return v;
 }
 // Lanes given to each of n items by a 256-thread workgroup: the largest power of two up to a wave.
-__device__ __forceinline__ int lanes_per(int n) {
+__host__ __device__ __forceinline__ int lanes_per(int n) {
   int l = 64;
   while (l > 1 && n * l > kGnThreads) l >>= 1;
   return l;
@@ -146,9 +146,11 @@ __device__ __forceinline__ int lanes_per(int n) {
 
 // Partial pairs of the chunks: a workgroup (chunk, block of channels) leaves one pair for each group
 // that it meets, part[(b * nchunk + chunk) * gy + block][ngb]. pair_total joins those of one group,
-// `lanes` lanes a group, each result in every lane.
+// `lanes` lanes a group, each result in every lane. A group that lies in two blocks of channels is joined by the
+// workgroups of both: `lanes`, and with it the order of the sum, is the same for all of them.
 struct GnParts {
   int gy, ngb, block_c;  // blocks of channels, pairs per block, channels per block
+  int lanes;
 };
 template <typename P2>
 __device__ __forceinline__ void pair_total(const P2* __restrict__ part, const GnParts& pt, const GnShape& s, int b, int g,
@@ -319,14 +321,15 @@ __global__ __launch_bounds__(kGnThreads) void gn_apply_kernel(GnMap x, GnShape s
 #pragma unroll
   for (int u = 0; u < kU; ++u) r[u] = *reinterpret_cast<const vec*>(src + min(p + u * l.R, p1 - 1) * x.sp);
   if (part) {
-    const int lanes = lanes_per(gr.ng), sub = static_cast<int>(threadIdx.x) & (lanes - 1);
+    const int lanes = pt.lanes, sub = static_cast<int>(threadIdx.x) & (lanes - 1);
     for (int gi = static_cast<int>(threadIdx.x) / lanes; gi < gr.ng; gi += kGnThreads / lanes) {
       double a, q;
       pair_total(part, pt, s, b, gr.g0 + gi, sub, lanes, a, q);
       if (sub == 0) {
         const double2 st = stat_of(a, q, static_cast<double>(s.HW) * s.cpg, eps);
         cg[gi] = lds_stat(st);
-        if (chunk == 0) stat[static_cast<long long>(b) * s.G + gr.g0 + gi] = st;
+        // by the block of its first channel alone
+        if (chunk == 0 && (gr.g0 + gi) * s.cpg >= gr.c0) stat[static_cast<long long>(b) * s.G + gr.g0 + gi] = st;
       }
     }
   } else {
@@ -551,7 +554,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_apply_kernel(GnMap x, GnMap
       keep(gi, v.x, v.y);
     }
   } else {
-    const int lanes = lanes_per(gr.ng), sub = static_cast<int>(threadIdx.x) & (lanes - 1);
+    const int lanes = pt.lanes, sub = static_cast<int>(threadIdx.x) & (lanes - 1);
     for (int gi = static_cast<int>(threadIdx.x) / lanes; gi < gr.ng; gi += kGnThreads / lanes) {
       double a, q;
       pair_total(gpart, pt, s, b, gr.g0 + gi, sub, lanes, a, q);
@@ -689,6 +692,7 @@ GnParts gn_parts(const GnShape& s, int V) {
   pt.gy = static_cast<int>(ceil_div(s.C, pt.block_c));
   const long long n = static_cast<long long>(pt.block_c) / s.cpg + 2;
   pt.ngb = static_cast<int>(n < s.G ? n : s.G);
+  pt.lanes = lanes_per(pt.ngb);
   return pt;
 }
 size_t gn_pairs(const GnShape& s, const GnParts& pt) { return static_cast<size_t>(s.B) * s.nchunk * pt.gy * pt.ngb; }
