@@ -1,7 +1,8 @@
 // norm.hip — group norm with an activation on channels-last maps (gfx950), forward and backward.
 //
 // For sample b and group g (M = HW * C / G values: the group's channels at every pixel)
-//   mean = sum x / M,  rstd = 1 / sqrt(sum x^2 / M - mean^2 + eps)          (sums in f64)
+//   mean = p + sum (x - p) / M,  rstd = 1 / sqrt(sum (x - p)^2 / M - (mean - p)^2 + eps)
+// with the pivot p, the group's first value, and sums in f64
 //   xh = (x - mean) rstd,  z = xh w[c] + beta[c],  y = act(z)
 // and with gz = gy act'(z), per channel S1 = sum_pixels gz, S2 = sum_pixels gz xh,
 //   g_w[c] = sum_b S2,  g_beta[c] = sum_b S1
@@ -168,9 +169,17 @@ __device__ __forceinline__ void pair_total(const P2* __restrict__ part, const Gn
   q = wave_part_sum(q, lanes);
 }
 
-// Partial sums of one chunk: (sum x, sum x^2) of each group that the workgroup's channels meet.
-// f64 from the first addition: the variance is a difference of the two, and sums of exact input
-// values keep it right for means up to 2^20 spreads; two f64 operations an element are far below
+// The first value of a group: what its sums are taken from. The variance is a difference of two sums, and a rounding
+// of one of them is as large as the mean's square: from 0 they lose the variance's f32 digits at means of 2^13
+// spreads and 8e-4 of it at 2^20. From a value of the group itself both sums are of the spread's size, or the
+// value lies so far out that it makes the variance.
+template <typename T>
+__device__ __forceinline__ double gn_pivot(const GnMap& x, const GnShape& s, int b, int g) {
+  return static_cast<double>(static_cast<float>(static_cast<const T*>(x.p)[b * x.sb + g * s.cpg]));
+}
+
+// Partial sums of one chunk: (sum x - p, sum (x - p)^2) of each group that the workgroup's channels meet.
+// f64 from the first subtraction on: three f64 operations an element are far below
 // the rate that would bound the kernel. 1 x 2048 x 129 x 257 bf16: 21.6 us, 6.3 TB/s. Maps of a few MB
 // (2 x 256 x 65 x 65 bf16: 4.3 us) are a launch and the latency of two rounds of loads.
 template <typename T, int V, int S>
@@ -181,10 +190,17 @@ __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(GnMap x, GnShape s
   const GnLane l = gn_lane<V>(s.C);
   const GnGroups gr = gn_groups<V>(l, s);
   typedef typename Raw<T, V>::type vec;
-  double sum[kN], sq[kN];
+  double sum[kN], sq[kN], pivot[kN];
 #pragma unroll
   for (int n = 0; n < kN; ++n) sum[n] = sq[n] = 0.0;
   if (l.on) {
+    const int c = gr.c0 + l.col * V;
+    int g = c / s.cpg;
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      if (c + n * S >= (g + 1) * s.cpg) ++g;  // a run lies in one group, the next run in the same or the next one
+      pivot[n] = gn_pivot<T>(x, s, b, g);
+    }
     const int p1 = min(s.HW, (chunk + 1) * s.ppc);
     const T* src = static_cast<const T*>(x.p) + b * x.sb + gr.c0 + l.col * V;
     int p = chunk * s.ppc + l.row;
@@ -193,7 +209,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(GnMap x, GnShape s
       unpack<T, V>(r, v);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const double d = static_cast<double>(v[i]);
+        const double d = static_cast<double>(v[i]) - pivot[i / S];
         sum[i / S] += d;
         sq[i / S] = fma(d, d, sq[i / S]);
       }
@@ -239,18 +255,18 @@ __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(GnMap x, GnShape s
   }
 }
 
-__device__ __forceinline__ double2 stat_of(double sum, double sq, double M, double eps) {
-  const double mean = sum / M;
-  double var = sq / M - mean * mean;
+__device__ __forceinline__ double2 stat_of(double sum, double sq, double M, double eps, double pivot) {
+  const double d = sum / M;
+  double var = sq / M - d * d;
   var = var < 0.0 ? 0.0 : var;  // NaN stays NaN
-  return make_double2(mean, 1.0 / sqrt(var + eps));
+  return make_double2(pivot + d, 1.0 / sqrt(var + eps));
 }
 
-// One workgroup per (group, sample): the chunks' partials joined. STATS: to mean and rstd. 3.8 to 4.8 us, a launch
-// and one chain of loads.
-template <typename P2, bool STATS>
-__global__ __launch_bounds__(kGnThreads) void gn_join_kernel(const P2* __restrict__ part, GnShape s, GnParts pt, double eps,
-                                                             double2* __restrict__ out) {
+// One workgroup per (group, sample): the chunks' partials joined. STATS: to mean and rstd of a map of T. 3.8 to 4.8 us,
+// a launch and one chain of loads.
+template <typename P2, bool STATS, typename T>
+__global__ __launch_bounds__(kGnThreads) void gn_join_kernel(GnMap x, const P2* __restrict__ part, GnShape s, GnParts pt,
+                                                             double eps, double2* __restrict__ out) {
   __shared__ double red[2][kGnThreads / 64];
   const int g = blockIdx.x, b = blockIdx.y, wave = static_cast<int>(threadIdx.x) >> 6;
   const int y0 = g * s.cpg / pt.block_c, ny = ((g + 1) * s.cpg - 1) / pt.block_c - y0 + 1;
@@ -269,7 +285,8 @@ __global__ __launch_bounds__(kGnThreads) void gn_join_kernel(const P2* __restric
   if (threadIdx.x == 0) {
     for (int w = 1; w < kGnThreads / 64; ++w) a += red[0][w], q += red[1][w];
     const long long i = static_cast<long long>(b) * s.G + g;
-    out[i] = STATS ? stat_of(a, q, static_cast<double>(s.HW) * s.cpg, eps) : make_double2(a, q);
+    if constexpr (STATS) out[i] = stat_of(a, q, static_cast<double>(s.HW) * s.cpg, eps, gn_pivot<T>(x, s, b, g));
+    else out[i] = make_double2(a, q);
   }
 }
 
@@ -326,7 +343,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_apply_kernel(GnMap x, GnShape s
       double a, q;
       pair_total(part, pt, s, b, gr.g0 + gi, sub, lanes, a, q);
       if (sub == 0) {
-        const double2 st = stat_of(a, q, static_cast<double>(s.HW) * s.cpg, eps);
+        const double2 st = stat_of(a, q, static_cast<double>(s.HW) * s.cpg, eps, gn_pivot<T>(x, s, b, gr.g0 + gi));
         cg[gi] = lds_stat(st);
         // by the block of its first channel alone
         if (chunk == 0 && (gr.g0 + gi) * s.cpg >= gr.c0) stat[static_cast<long long>(b) * s.G + gr.g0 + gi] = st;
@@ -748,8 +765,8 @@ extern "C" int protoseg_group_norm_fwd(const void* x, int x_dtype, int B, int HW
       hipLaunchKernelGGL((gn_stats_kernel<T, kV, kS>), grid, dim3(kGnThreads), 0, st, m, s, pt, part);
     }
     if (!inside)
-      hipLaunchKernelGGL((gn_join_kernel<double2, true>), dim3(static_cast<unsigned>(groups), static_cast<unsigned>(B)),
-                         dim3(kGnThreads), 0, st, part, s, pt, eps, stat);
+      hipLaunchKernelGGL((gn_join_kernel<double2, true, T>), dim3(static_cast<unsigned>(groups), static_cast<unsigned>(B)),
+                         dim3(kGnThreads), 0, st, m, part, s, pt, eps, stat);
     return gn_act(act_kind, [&](auto act) -> int {
       KernelTimer t("gn_apply_kernel", st);
       auto go = [&](auto kernel) {
@@ -803,8 +820,8 @@ extern "C" int protoseg_group_norm_bwd(const void* x, const void* g_y, int x_dty
                            st, m, mg, s, pt, stat, weight, bias, part, gpart);
       }
       if (!inside && g_x)
-        hipLaunchKernelGGL((gn_join_kernel<float2, false>), dim3(static_cast<unsigned>(groups), static_cast<unsigned>(B)),
-                           dim3(kGnThreads), 0, st, gpart, s, pt, 0.0, gsum);
+        hipLaunchKernelGGL((gn_join_kernel<float2, false, T>), dim3(static_cast<unsigned>(groups), static_cast<unsigned>(B)),
+                           dim3(kGnThreads), 0, st, m, gpart, s, pt, 0.0, gsum);
       const unsigned nsum = g_weight || g_bias ? static_cast<unsigned>(ceil_div(C, 16)) : 0u;
       KernelTimer t("gn_bwd_apply_kernel", st);
       auto go = [&](auto kernel) {

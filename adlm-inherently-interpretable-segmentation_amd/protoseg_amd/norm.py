@@ -6,8 +6,9 @@
 The reference's backbone normalises with BatchNorm and freezes it (segmentation/module.py:127),
 because its micro-batch of 2 crops (cityscapes_kld_imnet.gin:23) is too small for batch
 statistics; ``deeplab.DeepLabV2(norm="group")`` trains its normalisation at that batch with this
-operator instead. Statistics are formed in f64, so a mean far larger than the spread costs no
-accuracy, and all sums are joined in a fixed order (the same bits on every run).
+operator instead. Statistics are sums in f64 of differences to a value of the group itself, so a mean
+far larger than the spread (2^20 spreads in float32) costs no accuracy, and all sums are joined in a
+fixed order (the same bits on every run).
 
 A captured backward follows torch's rule for graphs: no eager autograd graph of the same leaves
 may be alive while it is captured.
