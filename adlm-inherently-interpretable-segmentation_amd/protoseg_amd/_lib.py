@@ -175,6 +175,17 @@ def call_on(index: int, name: str, *args) -> None:
         check(name, status)
 
 
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
+def direct(*tensors: torch.Tensor | None) -> bool:
+    """Whether a call may read these tensors' memory at once: no tracer, compiler, dispatch mode or tensor subclass
+    has to see it. Where one does, the call goes through its ``torch.library`` operator."""
+    if torch.compiler.is_compiling() or torch._C._is_tracing() or torch._C._len_torch_dispatch_stack():
+        return False
+    return all(t is None or type(t) in _PLAIN for t in tensors)
+
+
 def require_device(*tensors: torch.Tensor) -> torch.device:
     """All tensors on one ROCm device; the HIP path refuses CPU tensors loudly."""
     dev = None

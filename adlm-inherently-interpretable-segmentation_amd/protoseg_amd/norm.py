@@ -147,9 +147,55 @@ def group_norm_backward(x: Tensor, g_y: Tensor, weight: Optional[Tensor], bias: 
     return _backward(x, weight, bias, stats.contiguous(), (plan, at), g_y, groups, act, need_x, need_weight, need_bias)
 
 
+# The operators for tracers, compilers and dispatch modes. Other calls do without: an operator's dispatch costs a
+# training call more host time than the kernels take on the backbone's maps at the micro-batch of 2.
+@torch.library.custom_op("protoseg::group_norm", mutates_args=(), device_types="cuda")
+def _group_norm_op(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], groups: int, eps: float,
+                   act: int) -> Tuple[Tensor, Tensor]:
+    """group_norm_forward."""
+    return _forward(x, weight, bias, groups, eps, act)[:2]
+
+
+@_group_norm_op.register_fake
+def _(x, weight, bias, groups, eps, act):
+    return (torch.empty_like(x, memory_format=torch.channels_last),
+            x.new_empty((x.shape[0], groups, 2), dtype=torch.float64))
+
+
+@torch.library.custom_op("protoseg::group_norm_backward", mutates_args=(), device_types="cuda")
+def _group_norm_backward_op(x: Tensor, g_y: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], stats: Tensor, groups: int,
+                            act: int, need_x: bool, need_weight: bool, need_bias: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    """group_norm_backward; gradients that are not needed are empty."""
+    grads = group_norm_backward(x, g_y, weight, bias, stats, groups, act, need_x, need_weight, need_bias)
+    none = (x.dtype, torch.float32, torch.float32)
+    return tuple(x.new_empty(0, dtype=dt) if g is None else g for g, dt in zip(grads, none))
+
+
+@_group_norm_backward_op.register_fake
+def _(x, g_y, weight, bias, stats, groups, act, need_x, need_weight, need_bias):
+    C = x.shape[1]
+    return (torch.empty_like(x, memory_format=torch.channels_last) if need_x else x.new_empty(0),
+            x.new_empty(C if need_weight else 0, dtype=torch.float32), x.new_empty(C if need_bias else 0, dtype=torch.float32))
+
+
+def _op_setup(ctx, inputs, output):
+    x, weight, bias, groups, _, act = inputs
+    ctx.save_for_backward(x, weight, bias, output[1])
+    ctx.call = groups, act
+    ctx.mark_non_differentiable(output[1])
+
+
+def _op_backward(ctx, g_y, _):
+    x, weight, bias, stats = ctx.saved_tensors
+    need = ctx.needs_input_grad[:3]
+    grads = torch.ops.protoseg.group_norm_backward(x, g_y, weight, bias, stats, *ctx.call, *need)
+    return (*(g if n else None for g, n in zip(grads, need)), None, None, None)
+
+
+_group_norm_op.register_autograd(_op_backward, setup_context=_op_setup)
+
+
 class _GroupNorm(torch.autograd.Function):
-    # a Function and not a torch.library op as the layer's: its dispatch costs a training call more
-    # host time than the kernels take on the backbone's maps at the micro-batch of 2
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act):
         y, stats, used, plan = _forward(x, weight, bias, groups, eps, act)
@@ -184,6 +230,9 @@ def group_norm(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias: Op
     if bias is not None and bias.dtype != torch.float32 and bias.is_floating_point():
         bias = bias.float()
     args = (x, weight, bias, int(groups), float(eps), ACTIVATIONS[activation])
+    if not _lib.direct(x, weight, bias):
+        _lib.require_device(x, weight, bias)
+        return torch.ops.protoseg.group_norm(*args)[0]
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
         return _GroupNorm.apply(*args)

@@ -191,12 +191,19 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS,
     place, other layouts are copied once. The result is dense. Coefficients that let a singular value
     grow to 4 are refused.
     """
-    code = _matrix_dtype(g)
+    _matrix_dtype(g)
     if g.dim() < 2:
         raise _lib.ProtosegError(f"orthogonalize takes [..., rows, cols]; got {tuple(g.shape)}")
-    dev = _lib.require_device(g)
-    rows, cols = g.shape[-2:]
+    _lib.require_device(g)
     a, b, c = (float(v) for v in coefficients)
+    run = _orthogonalize if _lib.direct(g) else torch.ops.protoseg.orthogonalize
+    return run(g, int(steps), a, b, c, float(eps))
+
+
+def _orthogonalize(g: torch.Tensor, steps: int, a: float, b: float, c: float, eps: float) -> torch.Tensor:
+    """orthogonalize on the device's memory."""
+    code, dev = _matrix_dtype(g), g.device
+    rows, cols = g.shape[-2:]
     out = torch.empty(g.shape, dtype=g.dtype, device=dev)
     m = g if g.dim() == 3 else g.reshape(-1, rows, cols) if g.numel() else g.new_empty((0, rows, cols))
     count = m.shape[0]
@@ -207,9 +214,18 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS,
     lib = _lib.load()
     nbytes = lib.protoseg_orthogonalize_workspace_size(count, rows, cols)
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-    _lib.call_on(dev.index, "protoseg_orthogonalize", m.data_ptr(), code, count, rows, cols, stride, int(steps), a, b, c,
-                 float(eps), out.data_ptr(), ws.data_ptr(), nbytes)
+    _lib.call_on(dev.index, "protoseg_orthogonalize", m.data_ptr(), code, count, rows, cols, stride, steps, a, b, c, eps,
+                 out.data_ptr(), ws.data_ptr(), nbytes)
     return out
+
+
+# for tracers, compilers and dispatch modes
+_orthogonalize_op = torch.library.custom_op("protoseg::orthogonalize", _orthogonalize, mutates_args=(), device_types="cuda")
+
+
+@_orthogonalize_op.register_fake
+def _(g, steps, a, b, c, eps):
+    return g.new_empty(g.shape)
 
 
 class Muon(torch.optim.Optimizer):
