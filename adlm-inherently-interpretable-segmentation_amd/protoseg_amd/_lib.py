@@ -15,6 +15,7 @@ import pathlib
 import threading
 
 import torch  # noqa: F401  (must precede the CDLL load, see module docstring)
+from torch.autograd import forward_ad
 
 PACKAGE_ROOT = pathlib.Path(__file__).resolve().parent.parent
 CSRC_DIR = PACKAGE_ROOT / "csrc"
@@ -184,6 +185,14 @@ def direct(*tensors: torch.Tensor | None) -> bool:
     if torch.compiler.is_compiling() or torch._C._is_tracing() or torch._C._len_torch_dispatch_stack():
         return False
     return all(t is None or type(t) in _PLAIN for t in tensors)
+
+
+def refuse_tangents(what: str, *tensors: torch.Tensor | None) -> None:
+    """Forward-mode differentiation is refused: a kernel's result would drop the tangent."""
+    if forward_ad._current_level >= 0:  # a level of dual numbers is open
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ProtosegError(f"{what} has no forward-mode derivative")
 
 
 def require_device(*tensors: torch.Tensor) -> torch.device:

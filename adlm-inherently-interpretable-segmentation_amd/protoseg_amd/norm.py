@@ -219,12 +219,14 @@ def group_norm(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias: Op
 
     weight, bias: [C], float32 in the kernels (other floating types are widened, their gradients
     narrowed), or None. A channels-last x, and a slice of one along batch or channels, is read in
-    place; any other layout is copied once. Gradients with respect to x, weight and bias.
+    place; any other layout is copied once. Gradients with respect to x, weight and bias; second derivatives and
+    forward-mode derivatives are refused.
     """
     if activation not in ACTIVATIONS:
         raise _lib.ProtosegError(f"activation {activation!r} has no HIP kernel (one of {sorted(ACTIVATIONS)})")
     if not eps >= 0:
         raise _lib.ProtosegError(f"group norm eps {eps}")
+    _lib.refuse_tangents("group norm", x, weight, bias)
     if weight is not None and weight.dtype != torch.float32 and weight.is_floating_point():
         weight = weight.float()
     if bias is not None and bias.dtype != torch.float32 and bias.is_floating_point():

@@ -194,6 +194,7 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS,
     _matrix_dtype(g)
     if g.dim() < 2:
         raise _lib.ProtosegError(f"orthogonalize takes [..., rows, cols]; got {tuple(g.shape)}")
+    _lib.refuse_tangents("orthogonalize", g)
     _lib.require_device(g)
     a, b, c = (float(v) for v in coefficients)
     run = _orthogonalize if _lib.direct(g) else torch.ops.protoseg.orthogonalize
