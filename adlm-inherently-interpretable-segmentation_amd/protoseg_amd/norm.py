@@ -85,7 +85,7 @@ def _check_affine(name: str, t: Optional[Tensor], C: int, index: int) -> Optiona
 
 
 def _forward(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], groups: int, eps: float, act: int):
-    """y, stats and what a backward needs again: (x, weight, bias as read; the call's sizes)."""
+    """y, stats and what a backward needs again: (x, weight, bias) as read, and the call's sizes."""
     plan = _sizes(x.dtype, x.shape, groups)
     sizes, nbytes = plan[0], plan[1]
     if not 0 <= act < len(ACTIVATIONS):
@@ -103,13 +103,16 @@ def _forward(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], groups
         ws = x.new_empty(nbytes, dtype=torch.uint8)
         _lib.call_on(index, "protoseg_group_norm_fwd", x.data_ptr(), *sizes, *at, groups, _lib.addr(weight),
                      _lib.addr(bias), eps, act, y.data_ptr(), stats.data_ptr(), ws.data_ptr(), nbytes)
-    return y, stats, (x, weight, bias), (plan, at)
+    return y, stats, (x, weight, bias), plan
 
 
 def _backward(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], stats: Tensor, plan, g_y: Tensor, groups: int,
               act: int, need_x: bool, need_weight: bool, need_bias: bool):
-    """The backward on tensors that _forward returned; only g_y is new to it."""
-    (sizes, _, nbytes), at = plan
+    """The backward on the values that _forward returned. Their layout is looked up again: hooks on saved tensors (a
+    map kept in host memory meanwhile) may have given them another one."""
+    sizes, _, nbytes = plan
+    x, *at = _rows(x)
+    weight, bias = weight if weight is None else weight.contiguous(), bias if bias is None else bias.contiguous()
     C = sizes[3]
     g_x = torch.empty_like(x, memory_format=torch.channels_last) if need_x else None
     if sizes[1] == 0 or sizes[2] == 0:
@@ -118,6 +121,7 @@ def _backward(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], stats
     g_y, *g_at = _rows(g_y if g_y.dtype == x.dtype else g_y.to(x.dtype))
     g_w = x.new_empty(C, dtype=torch.float32) if need_weight else None
     g_b = x.new_empty(C, dtype=torch.float32) if need_bias else None
+    stats = stats.contiguous()
     ws = x.new_empty(nbytes, dtype=torch.uint8)
     _lib.call_on(x.get_device(), "protoseg_group_norm_bwd", x.data_ptr(), g_y.data_ptr(), *sizes, *at, *g_at, groups,
                  _lib.addr(weight), _lib.addr(bias), act, stats.data_ptr(), _lib.addr(g_x), _lib.addr(g_w), _lib.addr(g_b),
@@ -143,8 +147,7 @@ def group_norm_backward(x: Tensor, g_y: Tensor, weight: Optional[Tensor], bias: 
     if g_y.shape != x.shape or stats.dtype != torch.float64 or tuple(stats.shape) != (x.shape[0], groups, 2):
         raise _lib.ProtosegError("group norm backward: g_y and stats must be of the forward's shapes")
     weight, bias = _check_affine("weight", weight, C, x.get_device()), _check_affine("bias", bias, C, x.get_device())
-    x, *at = _rows(x)
-    return _backward(x, weight, bias, stats.contiguous(), (plan, at), g_y, groups, act, need_x, need_weight, need_bias)
+    return _backward(x, weight, bias, stats, plan, g_y, groups, act, need_x, need_weight, need_bias)
 
 
 # The operators for tracers, compilers and dispatch modes. Other calls do without: an operator's dispatch costs a
