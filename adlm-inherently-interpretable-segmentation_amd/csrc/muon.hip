@@ -1264,7 +1264,8 @@ struct NsMatrix {
   int rows, cols, count;
 };
 
-int pad_of(long long v) { return static_cast<int>((v + kPad - 1) / kPad * kPad); }
+long long pad64_of(long long v) { return (v + kPad - 1) / kPad * kPad; }
+int pad_of(long long v) { return static_cast<int>(pad64_of(v)); }  // of sizes that ns_check let pass
 
 // Groups of `mats` (at most kMaxGroups shapes, equal ones joined) and their buffers; returns the bytes in
 // all. which[i]: the group of mats[i]; index[i]: its first matrix there.
@@ -1337,7 +1338,7 @@ size_t ns_layout(NsGroups& gs, const std::vector<NsMatrix>& mats, std::vector<in
 int ns_check(int rows, int cols) {
   if (rows < 0 || cols < 0) return fail(PROTOSEG_ERR_INVALID, "orthogonalize: %d x %d matrix", rows, cols);
   const long long m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
-  if (static_cast<long long>(pad_of(m)) * pad_of(n) > (1LL << 29) || m > 16384)
+  if (pad64_of(m) * pad64_of(n) > (1LL << 29) || m > 16384)
     return fail(PROTOSEG_ERR_UNSUPPORTED, "orthogonalize: %d x %d matrix (at most 2^29 padded elements, 16384 in the smaller dimension)",
                 rows, cols);
   return PROTOSEG_OK;

@@ -187,6 +187,15 @@ def direct(*tensors: torch.Tensor | None) -> bool:
     return all(t is None or type(t) in _PLAIN for t in tensors)
 
 
+LARGEST = 0x7FFFFFFF  # size that the library's int arguments hold
+
+
+def check_sizes(what: str, *sizes: int) -> None:
+    """Refuses sizes that ctypes would cut to their low 32 bits."""
+    if any(n > LARGEST for n in sizes):
+        raise ProtosegError(f"{what} of sizes {sizes}: at most {LARGEST} each")
+
+
 def refuse_tangents(what: str, *tensors: torch.Tensor | None) -> None:
     """Forward-mode differentiation is refused: a kernel's result would drop the tangent."""
     if forward_ad._current_level >= 0:  # a level of dual numbers is open

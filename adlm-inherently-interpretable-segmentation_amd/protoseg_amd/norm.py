@@ -70,6 +70,8 @@ def _sizes(dtype: torch.dtype, shape: torch.Size, groups: int) -> Tuple[Tuple[in
     if groups < 1 or C < 1 or C % groups:
         raise _lib.ProtosegError(f"{C} channels do not divide into {groups} groups")
     sizes = (_CODES[dtype], B, H * W, C)
+    if B > 65535 or H * W > 1 << 30 or C > 1 << 20:
+        raise _lib.ProtosegError(f"group norm of {B} maps of {H * W} pixels and {C} channels (at most 65535, 2^30 and 2^20)")
     nbytes = _lib.load().protoseg_group_norm_workspace_size
     return sizes, nbytes(*sizes, groups, 0), nbytes(*sizes, groups, 1)
 

@@ -13,6 +13,7 @@ otherwise).
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import Dict, Iterable
 
 import torch
@@ -194,6 +195,8 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS,
     _matrix_dtype(g)
     if g.dim() < 2:
         raise _lib.ProtosegError(f"orthogonalize takes [..., rows, cols]; got {tuple(g.shape)}")
+    if g.numel() > _lib.LARGEST:
+        _lib.check_sizes("orthogonalize", math.prod(g.shape[:-2]), *g.shape[-2:])
     _lib.refuse_tangents("orthogonalize", g)
     _lib.require_device(g)
     a, b, c = (float(v) for v in coefficients)
@@ -275,6 +278,8 @@ class Muon(torch.optim.Optimizer):
                 n = p.numel()
                 if p.dtype != torch.float32 or p.grad.dtype != torch.float32 or p.grad.is_sparse or p.dim() < 2:
                     raise _lib.ProtosegError("protoseg Muon: float32 matrices and dense gradients only")
+                if n > _lib.LARGEST:
+                    _lib.check_sizes("Muon parameter", r, n // r)
                 st = self.state[p]
                 if "momentum_buffer" not in st:
                     if p.is_cuda and torch.cuda.is_current_stream_capturing():  # every replay would zero it again
