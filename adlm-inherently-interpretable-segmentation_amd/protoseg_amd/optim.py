@@ -243,7 +243,7 @@ class Muon(torch.optim.Optimizer):
     s = 0.2 sqrt(max(rows, cols)) (the update's root mean square then is about Adam's). Biases and other vectors belong to
     ``Adam``; ``train.PatchClassificationStep`` steps a list of optimizers. All tensors of a group share
     the launches, and a HIP graph holding ``step()`` replays as successive steps (after one step outside of it,
-    which makes the momentum). float32 on the GPU only.
+    which makes the momentum or brings a loaded one into the parameters' layout). float32 on the GPU only.
     """
 
     def __init__(self, params: Iterable, lr: float = 2e-2, momentum: float = 0.95, nesterov: bool = True,
@@ -281,16 +281,14 @@ class Muon(torch.optim.Optimizer):
                 if n > _lib.LARGEST:
                     _lib.check_sizes("Muon parameter", r, n // r)
                 st = self.state[p]
-                if "momentum_buffer" not in st:
-                    if p.is_cuda and torch.cuda.is_current_stream_capturing():  # every replay would zero it again
-                        raise _lib.ProtosegError("protoseg Muon: a captured step needs one step before it")
-                    st["momentum_buffer"] = torch.zeros_like(p)
-                buf, g = st["momentum_buffer"], p.grad
                 if not _dense_rows(p):
                     raise _lib.ProtosegError(f"protoseg Muon: parameter of strides {p.stride()} is not dense row by row")
-                if buf.stride() != p.stride() or buf.dtype != torch.float32 or buf.shape != p.shape:
-                    # (a loaded state of another layout) the columns of p, g and B have to be in one order
-                    buf = st["momentum_buffer"] = torch.empty_like(p).copy_(buf)
+                buf, g = st.get("momentum_buffer"), p.grad
+                if buf is None or buf.stride() != p.stride() or buf.dtype != torch.float32 or buf.shape != p.shape:
+                    # none yet, or a loaded state of another layout: the columns of p, g and B have to be in one order
+                    if p.is_cuda and torch.cuda.is_current_stream_capturing():  # every replay would make it anew
+                        raise _lib.ProtosegError("protoseg Muon: a captured step needs one step before it")
+                    buf = st["momentum_buffer"] = torch.zeros_like(p) if buf is None else torch.empty_like(p).copy_(buf)
                 if g.stride() != p.stride():
                     g = torch.empty_like(p).copy_(g)
                 if n:
