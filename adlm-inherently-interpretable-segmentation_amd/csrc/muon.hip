@@ -281,6 +281,7 @@ struct NsScale {
 __device__ __forceinline__ NsScale scale_of(double squares, float eps) {
   const double norm = sqrt(squares), all = norm + static_cast<double>(eps), part = norm / all;
   NsScale s;
+  if (all == 0.0) return NsScale{0.f, 0, 0};  // a zero matrix without eps: zeros
   s.small = part > 0.0 ? max(0, -ilogb(part) - 1) : 0;
   s.f = static_cast<float>(frexp(static_cast<double>(kScale) / all, &s.e));
   s.e += s.small;
