@@ -128,6 +128,12 @@ __device__ __forceinline__ long long at_pair(int row, int col, int ld) {
 struct Pair {
   _Float16 hi, lo;
 };
+// The compiler may join a product in v with the conversion to f16 and round it once there, and twice where it forms
+// hi again for lo: two different his. Products by powers of two are exact; others are pinned first.
+__device__ __forceinline__ float pinned(float v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
 __device__ __forceinline__ Pair split_pair(float v) {
   Pair p;
   p.hi = static_cast<_Float16>(v);
@@ -272,8 +278,9 @@ __global__ __launch_bounds__(kNormThreads) void ns_norm_kernel(NsGroups gs, NsIt
   }
 }
 
-// What takes an update's value to X0's: ldexpf(w f, e), kScale 2^small / (norm + eps) as a factor in [0.5, 1)
-// and a power of two, so that no f32 product leaves the range for any norm.
+// What takes an update's value to X0's: ldexpf(w, e) f, kScale 2^small / (norm + eps) as a factor in [0.5, 1)
+// and a power of two. The power comes first: it takes the largest values to some 2^11 for any norm, also from
+// f32's subnormals, where a product would round to few bits.
 struct NsScale {
   float f;
   int e, small;
@@ -326,7 +333,7 @@ __global__ __launch_bounds__(256) void ns_load_kernel(NsGroups gs, NsItems its, 
     float w = v[u];
     if constexpr (STEP) w = nesterov ? fmaf(mu, o[u], v[u]) : o[u];
     const bool in = r0 + lr + 4 * u < rows && c0 + lc < cols;
-    tile[lr + 4 * u][lc] = in ? ldexpf(w * sc.f, sc.e) : 0.f;
+    tile[lr + 4 * u][lc] = in ? ldexpf(w, sc.e) * sc.f : 0.f;
   }
   __syncthreads();
   _Float16* dst = pairs_of(gs, g, kX0, it.index + mat);
@@ -1029,7 +1036,7 @@ __global__ __launch_bounds__(kSmallThreads, 1) void ns_small_kernel(NsItems its,
       f16x8 hi, lo;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const Pair p = split_pair(ldexpf(v0[q][e] * sc.f, sc.e));
+        const Pair p = split_pair(pinned(ldexpf(v0[q][e], sc.e) * sc.f));
         hi[e] = p.hi;
         lo[e] = p.lo;
       }

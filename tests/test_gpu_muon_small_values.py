@@ -30,3 +30,16 @@ def test_a_zero_gradient_without_eps(device, shape):
     p.grad = torch.zeros_like(p)
     optim.Muon([p], lr=0.1, eps=0.0, weight_decay=0.5).step()
     assert torch.equal(p, torch.full_like(p, 1 - 0.1 * 0.5))
+
+
+@pytest.mark.parametrize("eps", [1e-7, 0.0, 2.0 ** -140])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_subnormal_values(device, shape, eps):
+    """Multiples of 2^-149 up to 8 of them, which f32 holds exactly. Where eps is far larger than the matrix, the
+    result is as small against 1 as X0 is, and the bound with it."""
+    from protoseg_amd import optim
+    gen = torch.Generator().manual_seed(2)
+    g = (torch.randint(-8, 9, shape, generator=gen).double() * 2.0 ** -149).float()
+    assert bool((g != 0).any()) and g.abs().max().item() < 2.0 ** -126
+    g = g.to(device)
+    check(optim.orthogonalize(g, eps=eps), g, eps=eps)
