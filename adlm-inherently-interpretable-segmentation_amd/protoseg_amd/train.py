@@ -96,6 +96,10 @@ def _default_kld(distances: Tensor, target_img: Tensor, class_identity: Tensor):
     return kld_with_pairs(distances, target_img, cols, int(class_identity.shape[1]), mpc)
 
 
+def _each(one_or_list):
+    return list(one_or_list) if isinstance(one_or_list, (list, tuple)) else [one_or_list]
+
+
 class PatchClassificationStep:
     """One training micro-step of module.py:_step ('train'), data-parallel when torch.distributed
     is initialised (or ``process_group`` is given) with more than one rank.
@@ -103,7 +107,8 @@ class PatchClassificationStep:
     ``ppnet(image)`` must return ``(logits [B, h, w, K], distances [B, P, h, w])`` or a list of
     such pairs (PPNet.forward with patch_classification). ``target`` is the label map at image
     resolution [B, H, W] (resized here with PIL-nearest semantics) or already at [B, h, w].
-    ``optimizer`` may be a list: each parameter in one of them, all stepped at the boundary.
+    ``optimizer`` may be a list: each parameter in one of them, all stepped at the boundary; ``lr_scheduler`` then
+    too, one or more for each (a scheduler changes the learning rates of its own optimizer alone).
     ``kld_fn(distances, target_img, class_identity) -> (mean loss, n_pairs)`` and
     ``resize_fn(labels, h, w)`` default to the HIP kernels.
     """
@@ -209,6 +214,7 @@ class PatchClassificationStep:
         self.buckets.wait()
         for opt in self.optimizers:
             opt.step()
-        if self.lr_scheduler is not None:
-            self.lr_scheduler.step()
+        for scheduler in _each(self.lr_scheduler):
+            if scheduler is not None:
+                scheduler.step()
         self.iter_steps = 0
