@@ -119,7 +119,6 @@ class PatchClassificationStep:
                  kld_fn: Optional[Callable] = None, resize_fn: Optional[Callable] = None):
         self.ppnet = ppnet
         self.optimizer = optimizer
-        self.optimizers = list(optimizer) if isinstance(optimizer, (list, tuple)) else [optimizer]
         self.loss_weight_crs_ent = loss_weight_crs_ent
         self.loss_weight_kld = loss_weight_kld
         self.loss_weight_l1 = loss_weight_l1
@@ -196,7 +195,7 @@ class PatchClassificationStep:
         if self.iter_steps == 0:
             # in place, as the reference's optimizer.zero_grad() (module.py:122; torch 1.10's
             # default): the gradients stay views into the exchange buckets' buffers
-            for opt in self.optimizers:
+            for opt in _each(self.optimizer):
                 opt.zero_grad(set_to_none=False)
         boundary = self.iter_steps + 1 == self.iter_size
         if boundary:
@@ -212,7 +211,7 @@ class PatchClassificationStep:
         """The accumulation boundary: gradient exchange (if not already overlapped), optimizer
         and scheduler step (module.py:238-243)."""
         self.buckets.wait()
-        for opt in self.optimizers:
+        for opt in _each(self.optimizer):
             opt.step()
         for scheduler in _each(self.lr_scheduler):
             if scheduler is not None:
