@@ -71,7 +71,11 @@ def muon_param_groups(ppnet, lr_matrices: float = 2e-3, lr_vectors: float = 2.5e
     """The joint phase's parameters (joint_param_groups) split for two optimizers: the matrices
     (convolution weights of the backbone and the add-on layers, prototype vectors) for
     ``optim.Muon``, and the rest (biases, group norm) for ``optim.Adam``. Pass both to
-    ``PatchClassificationStep(optimizer=[Muon(...), Adam(...)])``."""
+    ``PatchClassificationStep(optimizer=[Muon(...), Adam(...)])``.
+
+    One learning rate each: the 1x and 10x rates of joint_param_groups, which spare a pretrained backbone, are not
+    carried over (an orthogonalised update has one size for every matrix, and a group-norm backbone starts from
+    scratch). Weight decay is."""
     matrices, vectors = [], []
     for group in joint_param_groups(ppnet, weight_decay=weight_decay):
         for p in group["params"]:
