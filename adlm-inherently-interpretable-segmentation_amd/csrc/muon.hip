@@ -158,6 +158,7 @@ __device__ __forceinline__ void store_block(_Float16* dst, const Pair (&p)[16], 
 // (Stored from the registers it came in, 8 B down each column, a block took 4 times the cache lines.)
 __device__ __forceinline__ void mirror_block(Pair (&p)[16], unsigned lds, int lane) {
   const int j = lane & 31, h = lane >> 5;
+  wave_lds_fence();  // the sums that a caller read from here, of a type that the stores below need not wait for
 #pragma unroll
   for (int r = 0; r < 16; ++r)
     *reinterpret_cast<__attribute__((address_space(3))) unsigned*>(
