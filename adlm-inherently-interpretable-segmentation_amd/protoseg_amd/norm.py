@@ -134,6 +134,9 @@ def _backward(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], stats
 def group_norm_forward(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], groups: int, eps: float,
                        act: int) -> Tuple[Tensor, Tensor]:
     """(y in x's dtype, channels last; f64 [B, groups, 2] means and reciprocal deviations). No autograd."""
+    if not _lib.direct(x, weight, bias):
+        with torch.no_grad():
+            return torch.ops.protoseg.group_norm(x, weight, bias, groups, eps, act)
     return _forward(x, weight, bias, groups, eps, act)[:2]
 
 
@@ -141,6 +144,15 @@ def group_norm_backward(x: Tensor, g_y: Tensor, weight: Optional[Tensor], bias: 
                         act: int, need_x: bool = True, need_weight: bool = True,
                         need_bias: bool = True) -> Tuple[Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
     """Gradients of group_norm_forward's y with respect to (x, weight, bias); None where not needed."""
+    need = need_x, need_weight, need_bias
+    if not _lib.direct(x, g_y, weight, bias, stats):
+        with torch.no_grad():
+            grads = torch.ops.protoseg.group_norm_backward(x, g_y, weight, bias, stats, groups, act, *need)
+        return tuple(g if n else None for g, n in zip(grads, need))
+    return _checked_backward(x, g_y, weight, bias, stats, groups, act, *need)
+
+
+def _checked_backward(x, g_y, weight, bias, stats, groups, act, need_x, need_weight, need_bias):
     plan = _sizes(x.dtype, x.shape, groups)
     C = plan[0][3]
     if not 0 <= act < len(ACTIVATIONS):
@@ -171,7 +183,7 @@ def _(x, weight, bias, groups, eps, act):
 def _group_norm_backward_op(x: Tensor, g_y: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], stats: Tensor, groups: int,
                             act: int, need_x: bool, need_weight: bool, need_bias: bool) -> Tuple[Tensor, Tensor, Tensor]:
     """group_norm_backward; gradients that are not needed are empty."""
-    grads = group_norm_backward(x, g_y, weight, bias, stats, groups, act, need_x, need_weight, need_bias)
+    grads = _checked_backward(x, g_y, weight, bias, stats, groups, act, need_x, need_weight, need_bias)
     none = (x.dtype, torch.float32, torch.float32)
     return tuple(x.new_empty(0, dtype=dt) if g is None else g for g, dt in zip(grads, none))
 

@@ -81,3 +81,16 @@ def test_traced_orthogonalize(device):
     assert torch.equal(traced(other), optim.orthogonalize(other) * 2)
     leaf = g.clone().requires_grad_(True)
     assert not optim.orthogonalize(leaf).requires_grad
+
+
+def test_traced_calls_without_autograd(device):
+    from protoseg_amd import norm
+    x, w, b, gy = make(device, 2, 24, 9, 7, torch.float32, 84)
+
+    def both(x, gy):
+        y, stats = norm.group_norm_forward(x, w, b, 6, 1e-5, 3)
+        return (y, *norm.group_norm_backward(x, gy, w, b, stats, 6, 3))
+
+    x2, _, _, gy2 = make(device, 2, 24, 9, 7, torch.float32, 85)
+    traced = torch.jit.trace(both, (x, gy))
+    assert all(torch.equal(a, c) for a, c in zip(traced(x2, gy2), both(x2, gy2)))

@@ -23,6 +23,21 @@ def test_group_norm_is_an_operator_to_a_tracer():
             norm.group_norm(x, 2, activation="gelu")
 
 
+def test_the_calls_without_autograd_are_operators_too():
+    with FakeTensorMode():
+        x = torch.empty(2, 8, 5, 4, device="cuda:0").contiguous(memory_format=torch.channels_last)
+        w = torch.empty(8, device="cuda:0")
+
+        def both(x, w):
+            y, stats = norm.group_norm_forward(x, w, None, 2, 1e-5, 1)
+            gx, gw, gb = norm.group_norm_backward(x, y, w, None, stats, 2, 1, need_x=False)
+            assert gx is None and gw.shape == gb.shape == (8,)
+            return gw
+
+        names = targets(make_fx(both)(x, w))
+        assert "protoseg.group_norm.default" in names and "protoseg.group_norm_backward.default" in names
+
+
 def test_orthogonalize_is_an_operator_to_a_tracer():
     with FakeTensorMode():
         g = torch.empty(3, 40, 20, device="cuda:0", dtype=torch.bfloat16)
