@@ -822,12 +822,11 @@ __global__ __launch_bounds__(256) void ns_join_kernel(NsGroups gs, NsJobs js) {
 
 // ---- one workgroup per matrix ---------------------------------------------------------------------------
 
-// Matrices of up to 64 rows and 384 columns (padded): norm, X and all products of one matrix in one
-// workgroup, X and four 64 x 64 matrices in LDS (64 * 384 * 4 + 4 * 16 KiB = 160 KiB). Such a matrix is a
-// chain of some 20 products of about 1 us each, and a launch each costs 4 to 5 us: 361 x 64 f32 takes 35 us
-// for 92. What bounds it is the chain of LDS reads, MFMAs, LDS writes and barriers (a step 3.0 us, a Gram
-// matrix and Q X 3.3, load and store 9), so the blocks of a product lie on as many waves: 12 for 10 blocks
-// (8 waves, two of them with two blocks: 40 us).
+// Matrices of up to 64 rows and 384 columns (padded), whose phases are single steps: norm, X and all products of one
+// matrix in one workgroup, X and four 64 x 64 matrices in LDS (64 * 384 * 4 + 4 * 16 KiB = 160 KiB). Such a matrix is
+// a chain of 15 products of about 2 us each, and a launch each costs 4 to 5 us: 361 x 64 f32 takes 41 us. What
+// bounds it is the chain of LDS reads, MFMAs, LDS writes and barriers (a step 6.7 us, load and store 7.5), so the
+// blocks of a square lie on as many waves: 12 for 10 blocks.
 constexpr int kSmallM = 64, kSmallN = 384, kSmallThreads = 768;
 constexpr int kSmallSquare = 64 * 256;  // bytes of a 64 x 64 matrix of pairs
 
@@ -872,7 +871,11 @@ __device__ __forceinline__ void sm_cols(f16x8 (&f)[2], unsigned base, int pitch,
 #pragma unroll
   for (int t = 0; t < 2; ++t) f[t] = __builtin_bit_cast(f16x8, __builtin_shufflevector(v[t][0], v[t][1], 0, 1, 2, 3, 4, 5, 6, 7));
 }
-__device__ __forceinline__ void mma_pairs(f32x16& acc, f32x16& cross, const f16x8 (&l)[2], const f16x8 (&r)[2]) {
+// full: with lo lo, 2^-22 of the product, which the rounding of a long sum hides and that of a short one does not. Error
+// over that of f32 products without it and with it: 1.3 and 0.97 (8 x 16 to 8 x 128), 1.20 and 0.92 (32 x 64);
+// 19 x 361 takes 2.4 us more. Matrices of 64 rows have 0.96 of that error without it.
+__device__ __forceinline__ void mma_pairs(f32x16& acc, f32x16& cross, const f16x8 (&l)[2], const f16x8 (&r)[2], bool full) {
+  if (full) cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[1], r[1], cross, 0, 0, 0);
   cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[1], r[0], cross, 0, 0, 0);
   cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[0], r[1], cross, 0, 0, 0);
   acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[0], r[0], acc, 0, 0, 0);
@@ -883,10 +886,9 @@ __device__ __forceinline__ int anew(int v) {
   return v;
 }
 
-// The product L R^T of two symmetric 64 x 64 matrices that commute, so that it is symmetric too: the 10 blocks of
+// The square of a symmetric 64 x 64 matrix: the 10 blocks of
 // 16 x 16 on and above the diagonal, block w to wave w. A lane has column lane & 15 and rows 4 (lane >> 4) .. + 3
-// of its block. Blocks above the diagonal are stored with their mirror images: a result that is symmetric but for
-// its roundings drifts, to twice the error over five steps.
+// of its block. Blocks above the diagonal are stored with their mirror images.
 struct SmBlock {
   int r0, c0;
   bool on;
@@ -895,14 +897,15 @@ __device__ __forceinline__ SmBlock sm_block(int t) {
   const int bi = t < 4 ? 0 : t < 7 ? 1 : t < 9 ? 2 : 3, bc = t < 4 ? t : t < 7 ? t - 3 : t < 9 ? t - 5 : 3;
   return SmBlock{16 * bi, 16 * bc, t < 10};
 }
-__device__ __forceinline__ f32x4 sm_square(unsigned l, unsigned r, float mul, const SmBlock& bl, int lane) {
+__device__ __forceinline__ f32x4 sm_gram_square(unsigned a, float mul, const SmBlock& bl, int lane, bool full) {
   const int ln = anew(lane);
   f32x4 acc = {0.f, 0.f, 0.f, 0.f}, cross = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int st = 0; st < 2; ++st) {
     f16x8 lf[2], rf[2];
-    sm_rows16(lf, l, bl.r0, st, ln);
-    sm_rows16(rf, r, bl.c0, st, ln);
+    sm_rows16(lf, a, bl.r0, st, ln);
+    sm_rows16(rf, a, bl.c0, st, ln);
+    if (full) cross = __builtin_amdgcn_mfma_f32_16x16x32_f16(lf[1], rf[1], cross, 0, 0, 0);
     cross = __builtin_amdgcn_mfma_f32_16x16x32_f16(lf[1], rf[0], cross, 0, 0, 0);
     cross = __builtin_amdgcn_mfma_f32_16x16x32_f16(lf[0], rf[1], cross, 0, 0, 0);
     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(lf[0], rf[0], acc, 0, 0, 0);
@@ -1050,7 +1053,8 @@ __global__ __launch_bounds__(kSmallThreads, 1) void ns_small_kernel(NsItems its,
 
   const int bi = 32 * (wave & 1), bc = 32 * ((wave >> 1) & 1), part = wave >> 2;
   const SmBlock bl = sm_block(wave);
-  for (int p = 0, step = 0; p < pl.nphase; ++p) {
+  const bool full = m < kSmallM;
+  for (int p = 0; p < pl.nphase; ++p) {  // phases of one step (kind 0)
     {  // A = X X^T, a 32 x 32 block and every third 16 k a wave; the thirds meet in MT and MP
       f32x16 acc = zero16(), cross = zero16();
       const int ln = anew(lane);
@@ -1058,7 +1062,7 @@ __global__ __launch_bounds__(kSmallThreads, 1) void ns_small_kernel(NsItems its,
         f16x8 lf[2], rf[2];
         sm_rows(lf, X, xp, bi, st, ln);
         sm_rows(rf, X, xp, bc, st, ln);
-        mma_pairs(acc, cross, lf, rf);
+        mma_pairs(acc, cross, lf, rf, full);
       }
       const int mine = (wave & 3) * 1024 + lane;
       const lds_f32 *sum1 = lds_ptr<lds_f32>(MT) + mine, *sum2 = lds_ptr<lds_f32>(MP) + mine;
@@ -1094,44 +1098,25 @@ __global__ __launch_bounds__(kSmallThreads, 1) void ns_small_kernel(NsItems its,
       }
       __syncthreads();
     }
-    float sq = 0.f;
-    for (int i = 0; i < pl.phases[p]; ++i, ++step) {
-      const float sp = pl.sp[step];
-      const bool more = i + 1 < pl.phases[p];
-      const unsigned P = i == 0 ? MQ : MP;  // the first P is Q
-      f32x4 v, vq;
-      if (bl.on) {
-        v = sm_square(MA, MA, 1.f / (kScale * kScale), bl, lane);
-        const int ln = anew(lane);
-        const unsigned at = sm_mirror(MA, bl, ln);
-        const f16x4 ah = *lds_ptr<lds_f16x4>(at), al = *lds_ptr<lds_f16x4>(at ^ 64);
+    const float sp = pl.sp[p];
+    if (bl.on) {  // Q = a I + b A + c A A
+      f32x4 v = sm_gram_square(MA, 1.f / (kScale * kScale), bl, lane, full);
+      const int ln = anew(lane);
+      const unsigned at = sm_mirror(MA, bl, ln);
+      const f16x4 ah = *lds_ptr<lds_f16x4>(at), al = *lds_ptr<lds_f16x4>(at ^ 64);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = (static_cast<float>(ah[e]) + static_cast<float>(al[e])) * (1.f / kScale);
-          v[e] = fmaf(pl.c, v[e], pl.b * x);
-          if (bl.r0 + 4 * (ln >> 4) + e == bl.c0 + (ln & 15)) v[e] += pl.a;
-          v[e] *= sp;
-        }
-        sm_put(P, v, bl, lane);
+      for (int e = 0; e < 4; ++e) {
+        const float x = (static_cast<float>(ah[e]) + static_cast<float>(al[e])) * (1.f / kScale);
+        v[e] = fmaf(pl.c, v[e], pl.b * x);
+        if (bl.r0 + 4 * (ln >> 4) + e == bl.c0 + (ln & 15)) v[e] += pl.a;
+        v[e] *= sp;
       }
-      __syncthreads();
-      if (bl.on && more) {  // T = P A
-        v = sm_square(P, MA, 1.f / sp, bl, lane);
-        sm_put(MT, v, bl, lane);
-      }
-      if (bl.on && i > 0) vq = sm_square(P, MQ, pl.sq[step] / (sp * sq), bl, lane);  // Q <- P Q, stored once every wave has read Q
-      sq = i > 0 ? pl.sq[step] : sp;
-      __syncthreads();
-      if (bl.on && i > 0) sm_put(MQ, vq, bl, lane);
-      if (bl.on && more) {  // A <- T P (at the first step P is Q, which no wave stores then)
-        v = sm_square(MT, P, 1.f / sp, bl, lane);
-        sm_put(MA, v, bl, lane);
-      }
-      __syncthreads();
+      sm_put(MQ, v, bl, lane);
     }
+    __syncthreads();
     // X <- Q X, 32 columns a wave; a wave reads its columns whole before it writes them
     const bool last = p + 1 == pl.nphase;
-    const float mul = 1.f / (sq * kScale);
+    const float mul = 1.f / (sp * kScale);
     for (int c0 = 32 * wave; c0 < np; c0 += 32 * (kSmallThreads / 64)) {
       f32x16 acc[2], cross[2];
 #pragma unroll
@@ -1144,8 +1129,8 @@ __global__ __launch_bounds__(kSmallThreads, 1) void ns_small_kernel(NsItems its,
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           sm_rows(qf, MQ, 256, 32 * b, st, ln);
-          if (last && tall) mma_pairs(acc[b], cross[b], xf, qf);  // transposed: lanes along the result's rows
-          else mma_pairs(acc[b], cross[b], qf, xf);
+          if (last && tall) mma_pairs(acc[b], cross[b], xf, qf, full);  // transposed: lanes along the result's rows
+          else mma_pairs(acc[b], cross[b], qf, xf, full);
         }
       }
       if (!last) {
