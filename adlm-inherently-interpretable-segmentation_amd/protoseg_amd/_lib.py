@@ -176,15 +176,20 @@ def call_on(index: int, name: str, *args) -> None:
         check(name, status)
 
 
-_PLAIN = (torch.Tensor, torch.nn.Parameter)
+# (names of the module's own: a call's host time is what bounds small ones)
+_Tensor, _Parameter = torch.Tensor, torch.nn.Parameter
+_is_tracing, _dispatch_modes, _is_compiling = torch._C._is_tracing, torch._C._len_torch_dispatch_stack, torch.compiler.is_compiling
 
 
 def direct(*tensors: torch.Tensor | None) -> bool:
     """Whether a call may read these tensors' memory at once: no tracer, compiler, dispatch mode or tensor subclass
     has to see it. Where one does, the call goes through its ``torch.library`` operator."""
-    if torch.compiler.is_compiling() or torch._C._is_tracing() or torch._C._len_torch_dispatch_stack():
+    if _is_compiling() or _is_tracing() or _dispatch_modes():
         return False
-    return all(t is None or type(t) in _PLAIN for t in tensors)
+    for t in tensors:
+        if t is not None and type(t) is not _Tensor and type(t) is not _Parameter:
+            return False
+    return True
 
 
 LARGEST = 0x7FFFFFFF  # size that the library's int arguments hold

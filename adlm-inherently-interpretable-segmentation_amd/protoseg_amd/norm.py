@@ -87,7 +87,7 @@ def _check_affine(name: str, t: Optional[Tensor], C: int, index: int) -> Optiona
 
 
 def _forward(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], groups: int, eps: float, act: int):
-    """y, stats and what a backward needs again: (x, weight, bias) as read, and the call's sizes."""
+    """y, stats and what a backward needs again: (x, weight, bias) as read, and the call's sizes and x's layout."""
     plan = _sizes(x.dtype, x.shape, groups)
     sizes, nbytes = plan[0], plan[1]
     if not 0 <= act < len(ACTIVATIONS):
@@ -105,15 +105,16 @@ def _forward(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], groups
         ws = x.new_empty(nbytes, dtype=torch.uint8)
         _lib.call_on(index, "protoseg_group_norm_fwd", x.data_ptr(), *sizes, *at, groups, _lib.addr(weight),
                      _lib.addr(bias), eps, act, y.data_ptr(), stats.data_ptr(), ws.data_ptr(), nbytes)
-    return y, stats, (x, weight, bias), plan
+    return y, stats, (x, weight, bias), (plan, x.stride(), at)
 
 
 def _backward(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], stats: Tensor, plan, g_y: Tensor, groups: int,
               act: int, need_x: bool, need_weight: bool, need_bias: bool):
-    """The backward on the values that _forward returned. Their layout is looked up again: hooks on saved tensors (a
-    map kept in host memory meanwhile) may have given them another one."""
-    sizes, _, nbytes = plan
-    x, *at = _rows(x)
+    """The backward on the values that _forward returned. Hooks on saved tensors (a map kept in host memory meanwhile)
+    may have given them another layout."""
+    (sizes, _, nbytes), stride, at = plan
+    if x.stride() != stride:
+        x, *at = _rows(x)
     weight, bias = weight if weight is None else weight.contiguous(), bias if bias is None else bias.contiguous()
     C = sizes[3]
     g_x = torch.empty_like(x, memory_format=torch.channels_last) if need_x else None
@@ -161,7 +162,7 @@ def _checked_backward(x, g_y, weight, bias, stats, groups, act, need_x, need_wei
     if g_y.shape != x.shape or stats.dtype != torch.float64 or tuple(stats.shape) != (x.shape[0], groups, 2):
         raise _lib.ProtosegError("group norm backward: g_y and stats must be of the forward's shapes")
     weight, bias = _check_affine("weight", weight, C, x.get_device()), _check_affine("bias", bias, C, x.get_device())
-    return _backward(x, weight, bias, stats, plan, g_y, groups, act, need_x, need_weight, need_bias)
+    return _backward(x, weight, bias, stats, (plan, None, None), g_y, groups, act, need_x, need_weight, need_bias)
 
 
 # The operators for tracers, compilers and dispatch modes. Other calls do without: an operator's dispatch costs a
