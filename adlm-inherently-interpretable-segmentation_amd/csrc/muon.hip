@@ -58,11 +58,11 @@ __device__ __forceinline__ P* lds_ptr(unsigned at) {
 constexpr int kPad = 64;
 constexpr int kMaxGroups = 24, kMaxItems = 32, kMaxSteps = 32;
 constexpr float kScale = 1024.f;  // of X, A and T: entries below 16 (checked) stay below 2^14
-constexpr long long kThinTiles = 256;  // ns_thin_kernel's tiles at most: it has one workgroup a CU (22 matrices of 256, 792 tiles: 303 us for 195)
+constexpr long long kThinTiles = 256;  // ns_thin_kernel's tiles at most: it has one workgroup a CU (22 matrices of 256, 792 tiles: 313 us for 204)
 // Up to so many 64 x 64 tiles (one a CU), of contractions of 8 stages or more, the two halves of a contraction run
-// beside each other (one matrix of 1024 x 1024: 245 us for 275; 100 of 64 x 500, 2 stages: 119 us for 114).
+// beside each other (one matrix of 1024 x 1024: 236 us for 248; 60 of 128 x 500, 4 stages: 170 us for 164).
 constexpr long long kHalvesTiles = 256, kHalvesStages = 8;
-constexpr long long kApplyTiles = 384;  // from so many 128 x 128 tiles of Q X on, they beat 64 x 64 ones (backbone: 1178 us for 1236)
+constexpr long long kApplyTiles = 384;  // from so many 128 x 128 tiles of Q X on, they beat 64 x 64 ones (backbone: 1406 us for 1468)
 constexpr int kNormThreads = 256, kMaxChunks = 256;
 constexpr long long kNormLeast = 16384;  // elements per workgroup of the sums of squares
 
@@ -183,7 +183,7 @@ __device__ __forceinline__ float src_at(const void* p, long long i) {
 }
 
 // The group (item) of a workgroup: a binary search, since each probe is a scalar load that the next one
-// waits for (22 matrices of 256 x 1024: 185 us for 190 in order). first[] is an array of its own, two lines of
+// waits for (22 matrices of 256 x 1024: 204 us for 211 in order). first[] is an array of its own, two lines of
 // the arguments and not one per group.
 template <int N>
 __device__ __forceinline__ int place_of(const int (&first)[N], int blk) {
@@ -196,7 +196,7 @@ __device__ __forceinline__ int place_of(const int (&first)[N], int blk) {
 
 // A launch gives group g n = per matrix x count workgroups, rounded up to a multiple of 8, and XCD x (which runs
 // the workgroups i % 8 == x) the x-th eighth of them in order: neighbouring tiles of a matrix share operands,
-// and an XCD finds them in its own 4 MiB L2 (22 matrices of 256 x 1024: 193 us for 220). -1: past the end.
+// and an XCD finds them in its own 4 MiB L2 (22 matrices of 256 x 1024: 204 us for 236). -1: past the end.
 __device__ __forceinline__ int xcd_local(int b, int n) {
   const int chunk = (n + 7) >> 3, i = (b & 7) * chunk + (b >> 3);
   return i < n && (b >> 3) < chunk ? i : -1;
@@ -971,8 +971,8 @@ __global__ __launch_bounds__(kSmallThreads, 1) void ns_small_kernel(NsItems its,
     return SmRun{i, kc, tall ? 8 * kc * cols + i : i * cols + 8 * kc, tall ? cols : 1, n - 8 * kc,
                  static_cast<int>(threadIdx.x) + q * kSmallThreads < runs};
   };
-  // Whole runs of a wide matrix's aligned rows in 16-B loads (64 x 384 f32: 32.7 us
-  // for 42.1 us one by one).
+  // Whole runs of a wide matrix's aligned rows in 16-B loads (64 x 384 f32: 41 us
+  // for 51 one by one).
   typedef T vec8 __attribute__((ext_vector_type(8)));
   typedef float f32x8 __attribute__((ext_vector_type(8)));
   const bool vec = !tall && cols % 8 == 0 && ((reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(buf)) & 31) == 0;

@@ -180,8 +180,8 @@ __device__ __forceinline__ double gn_pivot(const GnMap& x, const GnShape& s, int
 
 // Partial sums of one chunk: (sum x - p, sum (x - p)^2) of each group that the workgroup's channels meet.
 // f64 from the first subtraction on: three f64 operations an element are far below
-// the rate that would bound the kernel. 1 x 2048 x 129 x 257 bf16: 21.6 us, 6.3 TB/s. Maps of a few MB
-// (2 x 256 x 65 x 65 bf16: 4.3 us) are a launch and the latency of two rounds of loads.
+// the rate that would bound the kernel. 1 x 2048 x 129 x 257 bf16: 22.2 us, 6.1 TB/s. Maps of a few MB
+// (2 x 256 x 65 x 65 bf16: 4.6 us) are a launch and the latency of two rounds of loads.
 template <typename T, int V, int S>
 __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(GnMap x, GnShape s, GnParts pt, double2* __restrict__ part) {
   constexpr int kN = V / S, kU = 8;
@@ -402,8 +402,9 @@ __device__ __forceinline__ float grad_z(float gy, float x, float d, float a, flo
 
 // Partial sums of one chunk, S1 = sum gz and S2 = sum gz xh: per channel (part, f32 rows [2][C] of
 // each workgroup), and weighted by w over each group (gpart). f32 inside a chunk, where a thread adds up
-// ppc / R values of mixed sign (8 to 67 in this library's maps, about 1024 / V at most); the chunks are joined
-// in f64. 32 x 64 x 65 x 65 f32: 14.7 us, 4.7 TB/s.
+// ppc / R values of mixed sign (8 to 67 in this library's maps, about 1024 / V at most), and its rows, up to 256, are
+// added after it; the chunks are joined
+// in f64. 32 x 64 x 65 x 65 f32: 15.5 us, 4.5 TB/s.
 template <typename T, int V, int S, int ACT>
 __global__ __launch_bounds__(kGnThreads) void gn_bwd_sums_kernel(GnMap x, GnMap gy, GnShape s, GnParts pt,
                                                                  const double2* __restrict__ stat,

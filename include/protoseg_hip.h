@@ -606,11 +606,10 @@ int protoseg_group_norm_bwd(const void* x, const void* g_y, int x_dtype, int B, 
  *   X <- a X + b (X X^T) X + c (X X^T)^2 X
  * (for rows > cols on the transpose), i.e. every singular value s goes to a s + b s^3 + c s^5.
  *   dtype  F32, BF16 or F16; out [count, rows, cols] dense, of the same dtype (may not overlap g)
- * Arithmetic: f32-class (f16 pairs, f32 accumulation) for every dtype, with the error of f32 products (1.3 times it
- * below 64 rows or columns); a 16-bit result is rounded once. A zero
- * matrix gives zeros; a value that is not finite makes its own matrix NaN. Coefficients under which a
- * singular value in [0, 1] could grow to 4 are refused (PROTOSEG_ERR_UNSUPPORTED). No atomics: the same bits
- * on every run. workspace: protoseg_orthogonalize_workspace_size(...) bytes (0 for matrices that one
+ * Arithmetic: f32-class (f16 pairs, f32 accumulation) for every dtype, with the error of f32 products at most (up to
+ * 1.5 times it below 64 rows or columns); a 16-bit result is rounded once. A zero matrix gives zeros, also without
+ * eps; a value that is not finite makes its own matrix NaN. Coefficients under which a singular value in [0, 1]
+ * could grow to 4 are refused (PROTOSEG_ERR_UNSUPPORTED). No atomics: the same bits on every run. workspace: protoseg_orthogonalize_workspace_size(...) bytes (0 for matrices that one
  * workgroup takes whole), 256-B aligned, of one call at a time.
  */
 size_t protoseg_orthogonalize_workspace_size(int count, int rows, int cols);
