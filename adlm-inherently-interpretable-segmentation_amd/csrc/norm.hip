@@ -401,17 +401,17 @@ __device__ __forceinline__ float grad_z(float gy, float x, float d, float a, flo
 }
 
 // Partial sums of one chunk, S1 = sum gz and S2 = sum gz xh: per channel (part, f32 rows [2][C] of
-// each workgroup), and weighted by w over each group (gpart). f32 inside a chunk, where a thread adds up
-// ppc / R values of mixed sign (8 to 67 in this library's maps, about 1024 / V at most), and its rows, up to 256, are
-// added after it; the chunks are joined
-// in f64. 32 x 64 x 65 x 65 f32: 15.5 us, 4.5 TB/s.
+// each workgroup), and weighted by w over each group (gpart). Sums in f64, rounded to f32
+// once a chunk: the values have mixed signs, and f32 chains left a gradient of few channels 3 times the error of
+// a tree of f32 sums (19 x 2 x 16 x 11). That costs the training calls' kernels 0.2 to 1.3 us of 35 to 55.
+// 32 x 64 x 65 x 65 f32: 15.8 us, 4.4 TB/s.
 template <typename T, int V, int S, int ACT>
 __global__ __launch_bounds__(kGnThreads) void gn_bwd_sums_kernel(GnMap x, GnMap gy, GnShape s, GnParts pt,
                                                                  const double2* __restrict__ stat,
                                                                  const float* __restrict__ w, const float* __restrict__ beta,
                                                                  float* __restrict__ part, float2* __restrict__ gpart) {
   constexpr int kU = 2;
-  __shared__ float red[2][kGnThreads * V];
+  __shared__ double red[2][kGnThreads * V];
   __shared__ float4 cg[gn_most_groups(V, S)];
   const int b = static_cast<int>(blockIdx.x) / s.nchunk, chunk = static_cast<int>(blockIdx.x) - b * s.nchunk;
   const GnLane l = gn_lane<V>(s.C);
@@ -433,9 +433,9 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_sums_kernel(GnMap x, GnMap 
   if (l.on) {
     GnCoef<V, S> k;
     load_coef<V, S>(k, cg, w, beta, c0, gr.g0, s);
-    float s1[V], s2[V];
+    double s1[V], s2[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
+    for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.0;
     auto add = [&](const vec& vx, const vec& vg) {
       float v[V], g[V];
       unpack<T, V>(vx, v);
@@ -444,8 +444,8 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_sums_kernel(GnMap x, GnMap 
       for (int i = 0; i < V; ++i) {
         const float d = (v[i] - k.mh[i / S]) - k.ml[i / S];
         const float gz = grad_z<ACT>(g[i], v[i], d, k.a[i], k.beta[i], stat, w, b, c0 + i, s);
-        s1[i] += gz;
-        s2[i] = fmaf(gz, d, s2[i]);
+        s1[i] += static_cast<double>(gz);
+        s2[i] = fma(static_cast<double>(gz), static_cast<double>(d), s2[i]);
       }
     };
     while (p < p1) {
@@ -475,15 +475,15 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_sums_kernel(GnMap x, GnMap 
   const int n = l.cb * V;
   float* out = part + static_cast<long long>(blockIdx.x) * 2 * s.C + gr.c0;
   for (int i = threadIdx.x; i < n; i += kGnThreads) {
-    float a = red[0][i], q = red[1][i];
+    double a = red[0][i], q = red[1][i];
     for (int r = 1; r < l.R; ++r) {
       a += red[0][r * n + i];
       q += red[1][r * n + i];
     }
-    q *= cg[(gr.c0 + i) / s.cpg - gr.g0].z;
-    out[i] = a;
-    out[s.C + i] = q;
-    const float wc = w ? w[gr.c0 + i] : 1.f;
+    q *= static_cast<double>(cg[(gr.c0 + i) / s.cpg - gr.g0].z);
+    out[i] = static_cast<float>(a);
+    out[s.C + i] = static_cast<float>(q);
+    const double wc = w ? static_cast<double>(w[gr.c0 + i]) : 1.0;
     red[0][i] = wc * a;
     red[1][i] = wc * q;
   }
@@ -492,14 +492,14 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_sums_kernel(GnMap x, GnMap 
   float2* gout = gpart + (static_cast<long long>(blockIdx.x) * pt.gy + blockIdx.y) * pt.ngb;
   for (int gi = static_cast<int>(threadIdx.x) / lanes; gi < gr.ng; gi += kGnThreads / lanes) {
     const int lo = max((gr.g0 + gi) * s.cpg, gr.c0) - gr.c0, hi = min((gr.g0 + gi + 1) * s.cpg, gr.c1) - gr.c0;
-    float a = 0.f, q = 0.f;
+    double a = 0.0, q = 0.0;
     for (int i = lo + sub; i < hi; i += lanes) {
       a += red[0][i];
       q += red[1][i];
     }
     a = wave_part_sum(a, lanes);
     q = wave_part_sum(q, lanes);
-    if (sub == 0) gout[gi] = make_float2(a, q);
+    if (sub == 0) gout[gi] = make_float2(static_cast<float>(a), static_cast<float>(q));
   }
 }
 
@@ -631,7 +631,8 @@ __global__ void gn_zero_kernel(float* a, float* b, int n) {
 // 257 x 257 bf16 50.2 us for 45.5), none below 4096 elements (3 x 150 x 33 x 47 f16: 20.4 us, with 16384
 // 29.7). Where every workgroup of the second pass would join more than 2048 pairs of a sample, shorter chunks cost
 // as much as they save: 16384 elements then (2 x 256 x 65 x 65 bf16: 34.2 us, with 4096 37.1).
-// None above 2^18 elements, which bounds the chains of gn_bwd_sums_kernel.
+// None above 2^18 elements: forward and backward of 600 x 8 x 256 x 256 bf16 991 us for 1075, of 1 x 64 x 2930 x 2930
+// 1700 for 1725.
 void gn_chunks(GnShape& s) {
   long long want = ceil_div(kGnTarget, s.B);
   const long long all = static_cast<long long>(s.HW) * s.C, inside = kGnJoinInside / 2 / s.G, enough = ceil_div(all, kGnEnough);
