@@ -404,7 +404,7 @@ __device__ __forceinline__ float grad_z(float gy, float x, float d, float a, flo
 // each workgroup), and weighted by w over each group (gpart). Sums in f64, rounded to f32
 // once a chunk: the values have mixed signs, and f32 chains left a gradient of few channels 3 times the error of
 // a tree of f32 sums (19 x 2 x 16 x 11). That costs the training calls' kernels 0.2 to 1.3 us of 35 to 55.
-// 32 x 64 x 65 x 65 f32: 15.8 us, 4.4 TB/s.
+// 32 x 64 x 65 x 65 f32: 15.4 us, 4.5 TB/s.
 template <typename T, int V, int S, int ACT>
 __global__ __launch_bounds__(kGnThreads) void gn_bwd_sums_kernel(GnMap x, GnMap gy, GnShape s, GnParts pt,
                                                                  const double2* __restrict__ stat,
