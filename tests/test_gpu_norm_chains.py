@@ -1,6 +1,6 @@
-"""Group norm's backward where its f32 chains are longest: 2^18 elements a workgroup, whose threads add up 1024 / V values
-each (V channels a vector) and whose 256 rows are joined one after the other. float64 on the GPU; a sum of f32 chains of
-n values errs by n u sum |value|, u = 2^-24."""
+"""Group norm's backward where a workgroup's sums are longest: 2^18 elements, whose threads add up 1024 / V values each (V
+channels a vector) and whose 256 rows are joined one after the other. float64 on the GPU; the bound is that of f32 chains
+of n values, n u sum |value| with u = 2^-24, which sums in 64 bits keep far below."""
 import pytest
 import torch
 
